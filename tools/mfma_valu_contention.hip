@@ -7,12 +7,12 @@
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int STEPS = 2048, REPS = 8;
-enum Op { NONE, VADD, VCMP_SGPR, VCNDMASK_SGPR, ACC_WRITE, ACC_READ, SALU, SNOP0, SNOP7, VMEM_LOAD, VMEM_STORE, LDS_READ, SSTORE, VMAX, NOPS };
+enum Op { NONE, VADD, VCMP_SGPR, VCNDMASK_SGPR, ACC_WRITE, ACC_READ, SALU, SNOP0, SNOP7, VMEM_LOAD, VMEM_STORE, LDS_READ, VMAX, NOPS };
 const char* names[] = {"none", "v_add_u32", "v_cmp_lt_f32 -> sgpr pair", "v_cndmask_b32 (sgpr mask)", "v_accvgpr_write", "v_accvgpr_read", "s_add_u32", "s_nop 0", "s_nop 7",
-                       "buffer_load_dwordx4", "buffer_store_dwordx4", "ds_read_b128", "s_store_dwordx2", "v_max_i32"};
+                       "buffer_load_dwordx4", "buffer_store_dwordx4", "ds_read_b128", "v_max_i32"};
 
 template <int OP, int K>
-__global__ __launch_bounds__(256, 1) void k(float* __restrict__ out, const float* __restrict__ in, unsigned long long* __restrict__ sout) {
+__global__ __launch_bounds__(256, 1) void k(float* __restrict__ out, const float* __restrict__ in) {
     __shared__ f32x4 lds[256];
     const int lane = threadIdx.x & 63;
     lds[threadIdx.x] = f32x4{1.f, 2.f, 3.f, 4.f};
@@ -30,9 +30,6 @@ __global__ __launch_bounds__(256, 1) void k(float* __restrict__ out, const float
     f32x4 ld = {0.f, 0.f, 0.f, 0.f};
     __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)in, 0, 0x7fffffff, 0x00020000);
     __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc((void*)(out + 65536), 0, 0x7fffffff, 0x00020000);
-    unsigned long long* sp = sout + (blockIdx.x * 4 + (threadIdx.x >> 6)) * 8;
-    sp = (unsigned long long*)__builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)sp) ;   // low half only: rebuilt below
-    unsigned long long spb = ((unsigned long long)sout & 0xffffffff00000000ull) | (unsigned long long)sp;
 #pragma unroll 1
     for (int rep = 0; rep < REPS; ++rep) {
 #pragma unroll 1
@@ -60,24 +57,22 @@ __global__ __launch_bounds__(256, 1) void k(float* __restrict__ out, const float
                             __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], x[2], x[3]}, ws, (int)((blockIdx.x * 256 + threadIdx.x) * 16), 0, 2);
                         }
                         if (OP == LDS_READ) ld = lds[(threadIdx.x + s) & 255];
-                        if (OP == SSTORE) asm volatile("s_store_dwordx2 %0, %1, 0x0" ::"s"(sm), "s"(spb) : "memory");
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
-    if (OP == SSTORE) asm volatile("s_dcache_wb" ::: "memory");
     out[blockIdx.x * 256 + threadIdx.x] = a16[0] + a16[5] + a16[10] + a16[15] + (float)(x[0] + x[1] + x[2] + x[3]) + ld[0] + ld[3] + (float)su + (float)(sm & 1);
 }
 
 template <int OP, int K>
-float run(float* out, const float* in, unsigned long long* sout, float base_ms) {
+float run(float* out, const float* in, float base_ms) {
     const int blocks = 256 * 4;
     hipEvent_t e0, e1; (void)hipEventCreate(&e0); (void)hipEventCreate(&e1);
-    k<OP, K><<<blocks, 256>>>(out, in, sout);
+    k<OP, K><<<blocks, 256>>>(out, in);
     (void)hipEventRecord(e0);
-    k<OP, K><<<blocks, 256>>>(out, in, sout);
+    k<OP, K><<<blocks, 256>>>(out, in);
     (void)hipEventRecord(e1); (void)hipEventSynchronize(e1);
     float ms; (void)hipEventElapsedTime(&ms, e0, e1);
     const double flop = (double)blocks * 4 * STEPS * 4 * REPS * 4096.0;
@@ -88,18 +83,17 @@ float run(float* out, const float* in, unsigned long long* sout, float base_ms) 
 }
 
 int main() {
-    float *out, *in; unsigned long long* sout;
-    (void)hipMalloc(&out, 64 << 20); (void)hipMalloc(&in, 1 << 20); (void)hipMalloc(&sout, 1 << 20);
+    float *out, *in;
+    (void)hipMalloc(&out, 64 << 20); (void)hipMalloc(&in, 1 << 20);
     (void)hipMemset(in, 0, 1 << 20);
-    (void)run<NONE, 0>(out, in, sout, 0.f);                       // warm-up (clocks, code objects)
-    const float base = run<NONE, 0>(out, in, sout, 0.f);         // the bare chain: what every other case is measured against
-    run<VADD, 4>(out, in, sout, base); run<VADD, 16>(out, in, sout, base);
-    run<VMAX, 4>(out, in, sout, base);
-    run<VCMP_SGPR, 4>(out, in, sout, base); run<VCNDMASK_SGPR, 4>(out, in, sout, base);
-    run<ACC_WRITE, 4>(out, in, sout, base); run<ACC_READ, 4>(out, in, sout, base);
-    run<SALU, 4>(out, in, sout, base); run<SALU, 16>(out, in, sout, base);
-    run<SNOP0, 4>(out, in, sout, base); run<SNOP7, 4>(out, in, sout, base);
-    run<VMEM_LOAD, 4>(out, in, sout, base); run<VMEM_STORE, 4>(out, in, sout, base); run<LDS_READ, 4>(out, in, sout, base);
-    run<SSTORE, 4>(out, in, sout, base);
+    (void)run<NONE, 0>(out, in, 0.f);                       // warm-up (clocks, code objects)
+    const float base = run<NONE, 0>(out, in, 0.f);         // the bare chain: what every other case is measured against
+    run<VADD, 4>(out, in, base); run<VADD, 16>(out, in, base);
+    run<VMAX, 4>(out, in, base);
+    run<VCMP_SGPR, 4>(out, in, base); run<VCNDMASK_SGPR, 4>(out, in, base);
+    run<ACC_WRITE, 4>(out, in, base); run<ACC_READ, 4>(out, in, base);
+    run<SALU, 4>(out, in, base); run<SALU, 16>(out, in, base);
+    run<SNOP0, 4>(out, in, base); run<SNOP7, 4>(out, in, base);
+    run<VMEM_LOAD, 4>(out, in, base); run<VMEM_STORE, 4>(out, in, base); run<LDS_READ, 4>(out, in, base);
     return 0;
 }
