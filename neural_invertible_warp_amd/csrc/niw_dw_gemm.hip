@@ -189,9 +189,8 @@ __global__ __launch_bounds__(64 * WN * WK) void dw_gemm_kernel(GemmBatch batch, 
                 // row sums of the dY operand: thread t < rows sums its row of the staged slice
                 const int nrows = bias_side == 1 ? TN : TK;
                 if (tid < nrows) {
-                    // two packed adds per 16-byte read (the halves of a ds_read_b128 are aligned register pairs: v_pk_add_f32 without
-                    // moves) and two scalar adds per step: 18 vector instructions where the scalar form compiled to ~45 -- and vector
-                    // instructions are paid in matrix-pipe time (tools/mfma_valu_contention.hip)
+                    // two running sums, even and odd columns: four adds per 16-byte read and no moves -- vector instructions are paid
+                    // in matrix-pipe time (tools/mfma_valu_contention.hip)
                     typedef float f32x2 __attribute__((ext_vector_type(2)));
                     const float* rowp = (bias_side == 1 ? As : Bs) + tid * kLdsStride;
                     f32x2 s2 = {0.f, 0.f};
@@ -656,14 +655,14 @@ struct HeadsArgs {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// acc += x * d (both halves by the SAME scalar d): the scalar is element SEL of the register pair `dpair` -- selected by op_sel, not
-// copied into a pair first.  The kernel shares its SIMDs with the matrix waves of the wide launch (fp32 MFMA and vector instructions of
-// one SIMD do not overlap, tools/mfma_valu_contention.hip) and has 64 registers, so its loop is written to the minimum: one
-// v_pk_fma_f32 per two products, buffer loads with scalar offsets (no address arithmetic), no moves.
+// acc += x * d (both halves by the SAME scalar d): the scalar is element SEL of the register pair `dpair`.  The kernel shares its SIMDs
+// with the matrix waves of the wide launch (fp32 MFMA and vector instructions of one SIMD do not overlap,
+// tools/mfma_valu_contention.hip) and has 64 registers, so its loop is written to the minimum: one v_fma_f32 per product, buffer loads
+// with scalar offsets (no address arithmetic), no moves.
 template <int SEL>
-__device__ __forceinline__ void pk_fma_bcast(f32x2& acc, f32x2 x, f32x2 dpair) {
-    if constexpr (SEL == 0) asm volatile("v_pk_fma_f32 %0, %1, %2, %0 op_sel_hi:[1,0,1]" : "+v"(acc) : "v"(x), "v"(dpair));
-    else asm volatile("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,1,0] op_sel_hi:[1,1,1]" : "+v"(acc) : "v"(x), "v"(dpair));
+__device__ __forceinline__ void fma_bcast(f32x2& acc, f32x2 x, f32x2 dpair) {
+    acc[0] = fmaf(x[0], dpair[SEL], acc[0]);
+    acc[1] = fmaf(x[1], dpair[SEL], acc[1]);
 }
 
 // Sum each of N per-lane values over the 64 lanes in ~3 N vector instructions instead of 6 N: at step s the lanes whose bit s is set keep
@@ -726,13 +725,13 @@ __device__ __forceinline__ void heads_body(rsrc_t rsX, rsrc_t rsD, long long mpa
             }
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                pk_fma_bcast<0>(acc[q][0][0], x[t][q].lo, d[t].lo);
-                pk_fma_bcast<0>(acc[q][0][1], x[t][q].hi, d[t].lo);
+                fma_bcast<0>(acc[q][0][0], x[t][q].lo, d[t].lo);
+                fma_bcast<0>(acc[q][0][1], x[t][q].hi, d[t].lo);
                 if constexpr (R == 3) {
-                    pk_fma_bcast<1>(acc[q][1][0], x[t][q].lo, d[t].lo);
-                    pk_fma_bcast<1>(acc[q][1][1], x[t][q].hi, d[t].lo);
-                    pk_fma_bcast<0>(acc[q][2][0], x[t][q].lo, d[t].hi);
-                    pk_fma_bcast<0>(acc[q][2][1], x[t][q].hi, d[t].hi);
+                    fma_bcast<1>(acc[q][1][0], x[t][q].lo, d[t].lo);
+                    fma_bcast<1>(acc[q][1][1], x[t][q].hi, d[t].lo);
+                    fma_bcast<0>(acc[q][2][0], x[t][q].lo, d[t].hi);
+                    fma_bcast<0>(acc[q][2][1], x[t][q].hi, d[t].hi);
                 }
             }
         }
