@@ -30,6 +30,27 @@ class AdamGroup(ctypes.Structure):
     _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("n", _i64), ("lr", _d), ("step", _i32), ("reserved", _i32)]
 
 
+class GradTensor(ctypes.Structure):
+    """niw_grad_tensor of include/niw.h"""
+    _fields_ = [("grad", _vp), ("out", _vp), ("n", _i64), ("dtype", _i32), ("out_dtype", _i32)]
+
+
+class AdamTensor(ctypes.Structure):
+    """niw_adam_tensor of include/niw.h"""
+    _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("master", _vp), ("n", _i64), ("param_dtype", _i32),
+                ("grad_dtype", _i32), ("group", _i32), ("reserved", _i32)]
+
+
+class AdamHyper(ctypes.Structure):
+    """niw_adam_hyper of include/niw.h"""
+    _fields_ = [("lr", _d), ("weight_decay", _d), ("step", _i32), ("reserved", _i32)]
+
+
+class AdamClip(ctypes.Structure):
+    """niw_adam_clip of include/niw.h"""
+    _fields_ = [("max_norm", _d), ("kind", _i32), ("skip_nonfinite", _i32), ("total", _vp), ("workspace", _vp), ("norm", _vp)]
+
+
 class TrainDesc(ctypes.Structure):
     """niw_train_desc of include/niw.h, field for field"""
     _fp = ctypes.POINTER(_f)
@@ -97,6 +118,13 @@ SIGNATURES = {
     "niw_render_fwd": (_i, [ctypes.POINTER(RenderDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "niw_adam_step": (_i, [_vp, _vp, _vp, _vp, _i64, _d, _d, _d, _d, _i, _vp, _vp]),
     "niw_adam_step_multi": (_i, [ctypes.POINTER(AdamGroup), _i, _d, _d, _d, _vp, _vp]),
+    "niw_grad_check": (_i, [_vp, _i64, _i]),
+    "niw_grad_workspace_doubles": (_i64, [_vp, _i64]),
+    "niw_grad_norm": (_i, [_vp, _i64, _i, _vp, _vp, _vp, _vp]),
+    "niw_grad_clip": (_i, [_vp, _i64, _i, _d, _vp, _vp, _vp, _vp]),
+    "niw_adam_check": (_i, [_vp, _i64, _i]),
+    "niw_adam_workspace_doubles": (_i64, [_vp, _i64]),
+    "niw_adam_step_tensors": (_i, [_vp, _i64, _vp, _i, _d, _d, _d, _vp, _vp, _vp, _vp]),
     "niw_train_step_prepare": (_i, []),
     "niw_train_step_workspace_floats": (_i64, [ctypes.POINTER(TrainDesc)]),
     "niw_train_step": (_i, [ctypes.POINTER(TrainDesc), _vp, _i, _i, _vp]),

@@ -272,6 +272,272 @@ def adam_step_multi(groups, beta1=0.9, beta2=0.999, eps=1e-8, hyper_dev=None):
         _lib.call("niw_adam_step_multi", arr, len(groups), float(beta1), float(beta2), float(eps), _p(hyper_dev), _stream())
 
 
+# ------------------------------------------------------------------------------------------
+# gradient norm, clipping and Adam over lists of many tensors
+# ------------------------------------------------------------------------------------------
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}         # enum niw_dtype (include/niw.h)
+NORMS = {2.0: 0, math.inf: 1}                                             # enum niw_norm_kind
+
+
+def _norm_kind(norm_type):
+    kind = NORMS.get(float(norm_type))
+    if kind is None:
+        raise _lib.NiwError(f"norm_type {norm_type!r}: 2 or math.inf")
+    return kind
+
+
+def _layout(t):
+    """the dimensions that say which element lies where: (size, stride) without those of size 1, outermost first"""
+    return tuple((n, s) for n, s in zip(t.shape, t.stride()) if n != 1)
+
+
+def _check_dense(t, name):
+    """every element of the tensor in one gap-free run of memory, in whatever order: an elementwise pass may then walk that run"""
+    if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES:
+        raise _lib.NiwError(f"{name}: expected a float32, bfloat16 or float16 tensor, got {type(t).__name__} {getattr(t, 'dtype', '')}")
+    if t.layout != torch.strided or t.is_neg():
+        raise _lib.NiwError(f"{name}: expected a strided tensor that holds its own values, got {t.layout}{', a negated view' if t.is_neg() else ''}")
+    if t.is_contiguous() or t.numel() == 0:
+        return
+    run = 1
+    for n, s in sorted(_layout(t), key=lambda d: d[1]):
+        if s != run:
+            raise _lib.NiwError(f"{name}: shape {tuple(t.shape)} with strides {t.stride()} has gaps or shares elements; pass a dense tensor")
+        run *= n
+
+
+def _check_same_layout(a, b, name):
+    if a.shape != b.shape or (_layout(a) != _layout(b) and a.numel() > 1):
+        raise _lib.NiwError(f"{name}: shape {tuple(b.shape)} strides {b.stride()} against {tuple(a.shape)} {a.stride()}; the elements of a pair have to "
+                            "lie in the same order")
+
+
+def _check_device(tensors, name):
+    """the one GPU all of them are on (None: an empty list)"""
+    devices = {t.device for t in tensors}
+    if len(devices) > 1:
+        raise _lib.NiwError(f"{name}: tensors on several devices ({', '.join(sorted(map(str, devices)))})")
+    device = devices.pop() if devices else None
+    if device is not None and device.type != "cuda":
+        raise _lib.NiwError(f"{name}: expected CUDA/HIP tensors, got {device}")
+    return device
+
+
+def _checked(name, *args):
+    lib = _lib.load()
+    if getattr(lib, name)(*args):
+        raise _lib.NiwError(lib.niw_last_error_string().decode())
+
+
+class TensorTable:
+    """What grad_norm / grad_total / clip_grads need to know of a list of tensors, gathered and checked once for tensors that stay where they
+    are (a gradient bucket's views, gradients that are zeroed rather than dropped).  A plain list in its place is gathered at every call.
+    tensors: float32 / bfloat16 / float16, mixed at will, each dense in any order, any length; None entries are left out.
+    out: for clip_grads, one tensor per entry that receives the clipped values (same shape and order, any of the types); None: in place.
+    The table speaks of the MEMORY the tensors had when it was built and keeps that memory alive; a tensor that is given other storage
+    afterwards (.grad re-created by a backward, .data re-assigned, .to()) is not followed: build a new table."""
+
+    def __init__(self, tensors, out=None):
+        tensors = list(tensors)
+        out = [None] * len(tensors) if out is None else list(out)
+        if len(out) != len(tensors):
+            raise _lib.NiwError(f"TensorTable: {len(tensors)} tensors and {len(out)} outputs")
+        pairs = [(t, o) for t, o in zip(tensors, out) if t is not None]
+        if len({o is None for _, o in pairs}) > 1:
+            raise _lib.NiwError("TensorTable: an output for some tensors only")
+        for i, (t, o) in enumerate(pairs):
+            _check_dense(t, f"tensor {i}")
+            if o is not None:
+                _check_dense(o, f"output {i}")
+                _check_same_layout(t, o, f"output {i}")
+        self.device = _check_device([x for p in pairs for x in p if x is not None], "TensorTable")
+        self.in_place = not pairs or pairs[0][1] is None
+        self.numel = sum(t.numel() for t, _ in pairs)
+        self._keep = [(x, x.untyped_storage()) for p in pairs for x in p if x is not None]
+        self._n = len(pairs)
+        self._c = (_lib.GradTensor * max(self._n, 1))()
+        for c, (t, o) in zip(self._c, pairs):
+            o = t if o is None else o
+            c.grad, c.out, c.n, c.dtype, c.out_dtype = t.data_ptr(), o.data_ptr(), t.numel(), DTYPES[t.dtype], DTYPES[o.dtype]
+        _checked("niw_grad_check", self._c, self._n, 0)
+        self._overlap = _lib.load().niw_grad_check(self._c, self._n, 1) and _lib.load().niw_last_error_string().decode()
+        if self._overlap and not self.in_place:
+            raise _lib.NiwError(self._overlap)
+        self._doubles = _lib.load().niw_grad_workspace_doubles(self._c, self._n)
+
+
+def _table(grads, out=None):
+    if isinstance(grads, TensorTable):
+        if out is not None:
+            raise _lib.NiwError("the outputs of a TensorTable are given when it is built")
+        return grads
+    if isinstance(grads, torch.Tensor):
+        grads, out = [grads], None if out is None else [out]
+    return TensorTable(grads, out)
+
+
+def _on(device):
+    """makes the list's GPU current for a launch (its stream and allocations are that GPU's)"""
+    if device is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def grad_total(grads, norm_type=2.0):
+    """-> [1] float64 on the GPU: the sum of squares of all elements (norm_type 2) or their largest magnitude (math.inf).  What ranks with
+    different shares of the gradients exchange (sum / maximum) before clip_grads / adam_step_tensors get it as `total`."""
+    table, kind = _table(grads), _norm_kind(norm_type)
+    with _on(table.device):
+        total = torch.empty(1, device=table.device or "cuda", dtype=torch.float64)
+        ws = torch.empty(table._doubles, device=total.device, dtype=torch.float64)
+        with timed("grad_norm", table.numel):
+            _lib.call("niw_grad_norm", table._c, table._n, kind, _p(ws), _p(total), None, _stream())
+    return total
+
+
+def grad_norm(grads, norm_type=2.0):
+    """The global norm of a list of tensors (a TensorTable, a list, one tensor) -> 0-d float32 on the GPU, no synchronisation.  The sum of
+    squares is held in 64 bits.  Outside the autograd tape, like everything of this section."""
+    table, kind = _table(grads), _norm_kind(norm_type)
+    with _on(table.device):
+        norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
+        ws = torch.empty(table._doubles, device=norm.device, dtype=torch.float64)
+        with timed("grad_norm", table.numel):
+            _lib.call("niw_grad_norm", table._c, table._n, kind, _p(ws), None, _p(norm), _stream())
+    return norm
+
+
+def _total(total, device):
+    if total is None:
+        return None
+    if not (isinstance(total, torch.Tensor) and total.is_cuda and total.dtype == torch.float64 and total.numel() == 1):
+        raise _lib.NiwError("total: the [1] float64 tensor of grad_total")
+    if device is not None and total.device != device:
+        raise _lib.NiwError(f"total is on {total.device}, the tensors on {device}")
+    return total
+
+
+def _max_norm(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise _lib.NiwError(f"max_norm={max_norm}: a number from 0 on (math.inf clips nothing)")
+    return max_norm
+
+
+def clip_grads(grads, max_norm, norm_type=2.0, out=None, total=None):
+    """Scale a list of gradients by min(1, max_norm / (norm + 1e-6)) -- in place, or into `out` (one tensor per entry, e.g. float32 views of a
+    bucket for bfloat16 gradients) -- and return the norm they had (0-d float32 on the GPU).  No synchronisation: the factor never visits
+    the host.  total: the grad_total of all ranks where this rank holds a share; None: the norm of `grads` itself.
+    In place nothing is written when nothing has to be clipped.  An infinite norm makes finite gradients 0, a NaN makes all of them NaN."""
+    table, kind, max_norm = _table(grads, out), _norm_kind(norm_type), _max_norm(max_norm)
+    if table._overlap:
+        raise _lib.NiwError(table._overlap)
+    total = _total(total, table.device)
+    with _on(table.device):
+        norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
+        ws = torch.empty(table._doubles, device=norm.device, dtype=torch.float64) if total is None else None
+        with timed("clip_grads", table.numel):
+            _lib.call("niw_grad_clip", table._c, table._n, kind, max_norm, _p(total), _p(ws), _p(norm), _stream())
+    return norm
+
+
+class AdamTable:
+    """What adam_step_tensors needs to know of its tensors, gathered and checked once (see TensorTable for what it keeps and does not follow).
+    groups: up to 8 dicts of lists of equal length
+        params      float32, or bfloat16 / float16 with `master`
+        grads       float32 / bfloat16 / float16; a None entry leaves its parameter out
+        exp_avg, exp_avg_sq     float32
+        master      float32 copies that the update runs on (half-precision parameters receive the rounded result), None for float32
+    The tensors of one entry have the same shape and the same order in memory."""
+
+    def __init__(self, groups):
+        groups = [dict(g) for g in groups]
+        if not 1 <= len(groups) <= 8:
+            raise _lib.NiwError(f"AdamTable: 1..8 groups (got {len(groups)})")
+        rows = []
+        for k, g in enumerate(groups):
+            lists = {key: g.pop(key, None) for key in ("params", "grads", "exp_avg", "exp_avg_sq", "master")}
+            if g:
+                raise _lib.NiwError(f"AdamTable: group {k} has unknown keys {sorted(g)}")
+            lists = {key: None if v is None else list(v) for key, v in lists.items()}
+            if any(lists[key] is None for key in ("params", "grads", "exp_avg", "exp_avg_sq")):
+                raise _lib.NiwError(f"AdamTable: group {k} needs params, grads, exp_avg and exp_avg_sq")
+            n = len(lists["params"])
+            if any(v is not None and len(v) != n for v in lists.values()):
+                raise _lib.NiwError(f"AdamTable: the lists of group {k} differ in length")
+            for i in range(n):
+                row = {key: None if v is None else v[i] for key, v in lists.items()}
+                if row["grads"] is None:
+                    continue
+                name = f"group {k} entry {i}"
+                for key, t in row.items():
+                    if t is None and key == "master":
+                        continue
+                    _check_dense(t, f"{name} {key}")
+                    if key not in ("params", "grads") and t.dtype != torch.float32:
+                        raise _lib.NiwError(f"{name} {key}: expected float32, got {t.dtype}")
+                    _check_same_layout(row["params"], t, f"{name} {key}")
+                if (row["params"].dtype == torch.float32) != (row["master"] is None):
+                    raise _lib.NiwError(f"{name}: a half-precision parameter needs a float32 master copy (updates below half a step of its type would be "
+                                        "lost), a float32 parameter has none")
+                rows.append((k, row))
+        tensors = [t for _, row in rows for t in row.values() if t is not None]
+        self.device = _check_device(tensors, "AdamTable")
+        self.n_groups = len(groups)
+        self.numel = sum(row["params"].numel() for _, row in rows)
+        self._keep = [(t, t.untyped_storage()) for t in tensors]
+        self._n = len(rows)
+        self._c = (_lib.AdamTensor * max(self._n, 1))()
+        for c, (k, row) in zip(self._c, rows):
+            c.param, c.grad, c.exp_avg, c.exp_avg_sq = (row[key].data_ptr() for key in ("params", "grads", "exp_avg", "exp_avg_sq"))
+            c.master = None if row["master"] is None else row["master"].data_ptr()
+            c.n, c.param_dtype, c.grad_dtype, c.group = row["params"].numel(), DTYPES[row["params"].dtype], DTYPES[row["grads"].dtype], k
+        _checked("niw_adam_check", self._c, self._n, self.n_groups)
+        self._doubles = _lib.load().niw_adam_workspace_doubles(self._c, self._n)
+
+
+def _per_group(value, n, name, kind):
+    values = list(value) if isinstance(value, (list, tuple)) else [value] * n
+    if len(values) != n:
+        raise _lib.NiwError(f"{name}: {len(values)} values for {n} groups")
+    return [kind(v) for v in values]
+
+
+def adam_step_tensors(tensors, lr, step, weight_decay=0.0, beta1=0.9, beta2=0.999, eps=1e-8, max_norm=None, norm_type=2.0, skip_nonfinite=False, total=None,
+                      hyper_dev=None, decay_dev=None):
+    """Adam with decoupled weight decay over an AdamTable (or its list of groups), the arithmetic of adam_step.  lr, step (1-based) and
+    weight_decay: one value, or one per group.
+    max_norm: the update is made by min(1, max_norm / (norm + 1e-6)) times the gradients, norm = their global norm over all groups (or that of
+    `total`, see clip_grads); the clipped gradients are never written.  -> the norm (0-d float32 on the GPU), None without max_norm.
+    skip_nonfinite (with max_norm): a norm that is not finite leaves everything as it was -- decided on the GPU, the host's step counts on.
+    hyper_dev [n_groups, 2] = adam_hyper(lr, step) and decay_dev [n_groups] = lr * weight_decay (float32 device tensors): read by the kernel at
+    run time instead of lr / step / weight_decay (graph replays)."""
+    table = tensors if isinstance(tensors, AdamTable) else AdamTable(tensors)
+    n = table.n_groups
+    lr, step, decay = _per_group(lr, n, "lr", float), _per_group(step, n, "step", int), _per_group(weight_decay, n, "weight_decay", float)
+    for t, shape, name in ((hyper_dev, 2 * n, "hyper_dev"), (decay_dev, n, "decay_dev")):
+        if t is not None and (_f32(t, name) is not t or t.numel() != shape or t.device != (table.device or t.device)):
+            raise _lib.NiwError(f"{name}: a contiguous float32 tensor of {shape} values on the parameters' device")
+    hyper = (_lib.AdamHyper * n)(*[_lib.AdamHyper(lr=a, weight_decay=b, step=c) for a, b, c in zip(lr, decay, step)])
+    if max_norm is None:
+        if skip_nonfinite or total is not None:
+            raise _lib.NiwError("adam_step_tensors: skip_nonfinite and total go with max_norm (math.inf clips nothing)")
+        with _on(table.device), timed("adam", table.numel):
+            _lib.call("niw_adam_step_tensors", table._c, table._n, hyper, n, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev), None, _stream())
+        return None
+    total, kind, max_norm = _total(total, table.device), _norm_kind(norm_type), _max_norm(max_norm)
+    with _on(table.device):
+        norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
+        ws = torch.empty(table._doubles, device=norm.device, dtype=torch.float64) if total is None else None
+        clip = _lib.AdamClip(max_norm=max_norm, kind=kind, skip_nonfinite=1 if skip_nonfinite else 0, total=None if total is None else total.data_ptr(),
+                             workspace=None if ws is None else ws.data_ptr(), norm=norm.data_ptr())
+        with timed("adam", table.numel):
+            _lib.call("niw_adam_step_tensors", table._c, table._n, hyper, n, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev),
+                      ctypes.byref(clip), _stream())
+    return norm
+
+
 def pack_index(device):
     """gather table of the packed fp32 weight layout (architecture constant, built once per device)"""
     key = str(device)

@@ -1,0 +1,205 @@
+"""CPU: what the operators over lists of many tensors (gradient norm, clipping, Adam under the clip) refuse, at the C boundary and in the
+Python wrappers.  Nothing is launched: every check runs on the host, in front of the first launch."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from neural_invertible_warp_amd import _lib, ops
+
+
+def err():
+    return _lib.load().niw_last_error_string().decode()
+
+
+def grads(*rows):
+    a = (_lib.GradTensor * max(len(rows), 1))()
+    for c, (g, o, n, d, od) in zip(a, rows):
+        c.grad, c.out, c.n, c.dtype, c.out_dtype = g, o, n, d, od
+    return a
+
+
+@pytest.mark.parametrize("row,what", [
+    ((None, None, 4, 0, 0), "null pointer"),
+    ((1024, 1024, -1, 0, 0), "n=-1"),
+    ((1024, 1024, 1 << 60, 0, 0), "n="),
+    ((1024, 1024, 4, 3, 0), "dtype 3"),
+    ((1026, 1026, 4, 0, 0), "aligned"),
+    ((1025, 1025, 4, 1, 1), "aligned"),
+])
+def test_c_norm_and_clip_refuse_a_bad_descriptor(row, what):
+    lib = _lib.load()
+    a = grads(row)
+    for rc in (lib.niw_grad_check(a, 1, 0), lib.niw_grad_norm(a, 1, 0, 4096, 4096, None, None), lib.niw_grad_clip(a, 1, 0, 1.0, None, 4096, None, None)):
+        assert rc == -1 and what in err()
+
+
+@pytest.mark.parametrize("rows,what", [
+    ([(1024, None, 4, 0, 0)], "null pointer in output"),
+    ([(1024, 2048, 4, 0, 7)], "dtype 7"),
+    ([(1024, 2050, 4, 0, 0)], "aligned"),
+    ([(1024, 1024, 4, 1, 0)], "changes its type"),
+])
+def test_c_clip_refuses_a_bad_output(rows, what):
+    lib = _lib.load()
+    assert lib.niw_grad_clip(grads(*rows), len(rows), 0, 1.0, None, 4096, None, None) == -1 and what in err()
+    assert lib.niw_grad_check(grads(*rows), len(rows), 1) == -1 and what in err()
+
+
+@pytest.mark.parametrize("rows,ok", [
+    ([(1024, 1024, 4, 0, 0), (1040, 1040, 4, 0, 0)], True),                  # neighbours that touch
+    ([(1024, 1024, 4, 0, 0), (1024, 1024, 4, 0, 0)], False),                 # the same tensor twice
+    ([(1024, 1024, 4, 0, 0), (1036, 1036, 4, 0, 0)], False),                 # one element shared
+    ([(1024, 2048, 4, 0, 0), (1024, 4096, 4, 0, 0)], True),                  # one gradient into two outputs
+    ([(1024, 2048, 4, 0, 0), (4096, 2060, 4, 0, 0)], False),                 # outputs that overlap
+    ([(1024, 1028, 4, 0, 0)], False),                                        # an output that runs over its own gradient
+    ([(1024, 2048, 4, 1, 0), (2056, 8192, 4, 1, 0)], False),                 # an output over another gradient
+    ([(1024, 1024, 400, 0, 0), (1100, 4096, 1, 0, 0)], False),               # a gradient inside another that is written
+    ([(1024, 1024, 0, 0, 0), (1024, 1024, 0, 0, 0)], True),                  # nothing at the same place
+    ([(8192, 8192, 4, 0, 0), (1024, 1024, 4000, 0, 0)], False),              # a long one from before
+])
+def test_c_overlap_check(rows, ok):
+    lib = _lib.load()
+    rc = lib.niw_grad_check(grads(*rows), len(rows), 1)
+    assert (rc == 0) == ok and (ok or "overlap" in err())
+    assert lib.niw_grad_check(grads(*rows), len(rows), 0) == 0               # the norm may read whatever it likes
+
+
+def test_c_norm_and_clip_refuse_bad_arguments():
+    lib = _lib.load()
+    a = grads((1024, 1024, 4, 0, 0))
+    assert lib.niw_grad_norm(a, 1, 2, 4096, 4096, None, None) == -1 and "kind 2" in err()
+    assert lib.niw_grad_norm(a, 1, 0, None, 4096, None, None) == -1 and "null pointer" in err()
+    assert lib.niw_grad_norm(a, 1, 0, 4096, None, None, None) == -1 and "null pointer" in err()
+    assert lib.niw_grad_norm(a, -1, 0, 4096, 4096, None, None) == -1 and "-1 tensors" in err()
+    assert lib.niw_grad_norm(None, 1, 0, 4096, 4096, None, None) == -1 and "null pointer" in err()
+    for bad in (-1.0, math.nan, -math.inf):
+        assert lib.niw_grad_clip(a, 1, 0, bad, None, 4096, None, None) == -1 and "max_norm" in err()
+    assert lib.niw_grad_clip(a, 1, 5, 1.0, None, 4096, None, None) == -1 and "kind 5" in err()
+    assert lib.niw_grad_clip(a, 1, 0, 1.0, None, None, None, None) == -1 and "null pointer" in err()
+
+
+def adam_row(**kw):
+    r = _lib.AdamTensor(param=1024, grad=2048, exp_avg=4096, exp_avg_sq=8192, master=None, n=4, param_dtype=0, grad_dtype=0, group=0)
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return (_lib.AdamTensor * 1)(r)
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(param=None), "null pointer"), (dict(grad=None), "null pointer"), (dict(exp_avg=None), "null pointer"), (dict(exp_avg_sq=None), "null pointer"),
+    (dict(n=-4), "n=-4"), (dict(param_dtype=5, master=16384), "dtype 5"), (dict(grad_dtype=-1), "dtype 0 / -1"), (dict(group=1), "group 1 of 1"),
+    (dict(group=-1), "group -1"), (dict(master=16384), "master copy"), (dict(param_dtype=1), "master copy"), (dict(exp_avg=4098), "aligned"),
+    (dict(param_dtype=1, master=16385), "aligned"),
+])
+def test_c_adam_refuses_a_bad_descriptor(change, what):
+    lib = _lib.load()
+    h = (_lib.AdamHyper * 1)(_lib.AdamHyper(lr=1e-3, step=1))
+    assert lib.niw_adam_check(adam_row(**change), 1, 1) == -1 and what in err()
+    assert lib.niw_adam_step_tensors(adam_row(**change), 1, h, 1, 0.9, 0.999, 1e-8, None, None, None, None) == -1 and what in err()
+
+
+def test_c_adam_refuses_bad_arguments_and_overlaps():
+    lib = _lib.load()
+    row = adam_row()
+    step = lambda h, n=1, b1=0.9, b2=0.999, eps=1e-8, hd=None, dd=None, clip=None: lib.niw_adam_step_tensors(row, 1, h, n, b1, b2, eps, hd, dd, clip, None)
+    H = lambda **kw: (_lib.AdamHyper * 1)(_lib.AdamHyper(**{**dict(lr=1e-3, weight_decay=0.0, step=1), **kw}))
+    assert step(None) == -1 and "null pointer" in err()
+    assert step(H(), n=0) == -1 and "1..8 groups" in err()
+    assert step(H(), n=9) == -1 and "1..8 groups" in err()
+    assert step(H(step=0)) == -1 and "step=0" in err()
+    assert step(H(lr=math.nan)) == -1 and "lr=" in err()
+    assert step(H(weight_decay=-0.1)) == -1 and "weight_decay" in err()
+    assert step(H(weight_decay=0.1), hd=64) == -1 and "decay_dev" in err()
+    for kw in (dict(b1=1.0), dict(b2=1.0), dict(b1=-0.1), dict(eps=-1e-8), dict(b2=math.nan)):
+        assert step(H(), **kw) == -1 and "beta1" in err()
+    clip = lambda **kw: ctypes.byref(_lib.AdamClip(**{**dict(max_norm=1.0, kind=0, workspace=4096), **kw}))
+    assert step(H(), clip=clip(max_norm=-1.0)) == -1 and "max_norm" in err()
+    assert step(H(), clip=clip(kind=9)) == -1 and "kind 9" in err()
+    assert step(H(), clip=clip(workspace=None)) == -1 and "null pointer" in err()
+    for kw in (dict(exp_avg=1024), dict(exp_avg_sq=4100), dict(grad=1024), dict(param_dtype=1, master=1028)):
+        assert lib.niw_adam_check(adam_row(**kw), 1, 1) == -1 and "overlap" in err()
+
+
+def test_workspace_queries_are_host_arithmetic():
+    lib = _lib.load()
+    assert lib.niw_grad_workspace_doubles(None, 0) >= 1
+    small = lib.niw_grad_workspace_doubles(grads((1024, 1024, 4, 0, 0)), 1)
+    assert 1 <= small <= lib.niw_grad_workspace_doubles(grads((1024, 1024, 1 << 34, 0, 0)), 1)
+    assert lib.niw_adam_workspace_doubles(adam_row(n=1 << 33), 1) >= 1
+
+
+# ------------------------------------------------------------------------------------------ Python wrappers (CPU tensors: refused last)
+def z(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("tensors,out,what", [
+    ([z(4, dtype=torch.float64)], None, "float64"),
+    ([z(4, dtype=torch.int32)], None, "int32"),
+    ([3.0], None, "float"),
+    ([z(8)[::2]], None, "gaps"),
+    ([z(1, 4).expand(3, 4)], None, "shares"),
+    ([z(4, 6)[:, :3]], None, "gaps"),
+    ([z(4).to_sparse()], None, "sparse"),
+    ([z(4)], [], "1 tensors and 0 outputs"),
+    ([z(4), z(4)], [z(4), None], "some tensors only"),
+    ([z(4)], [z(5)], "same order"),
+    ([z(4, 6)], [z(6, 4).t()], "same order"),
+    ([z(4)], [z(4, dtype=torch.int64)], "int64"),
+    ([torch._neg_view(z(4))], None, "negated"),
+    ([z(4)], None, "expected CUDA/HIP"),
+    ([z(0)], None, "expected CUDA/HIP"),
+])
+def test_tensor_table_refuses(tensors, out, what):
+    with pytest.raises(_lib.NiwError, match=what):
+        ops.TensorTable(tensors, out=out)
+
+
+def test_none_entries_are_left_out_before_any_check():
+    with pytest.raises(_lib.NiwError, match="expected CUDA/HIP"):
+        ops.TensorTable([None, z(4)], out=[None, z(4)])
+
+
+@pytest.mark.parametrize("call,what", [
+    (lambda t: ops.grad_norm(t, norm_type=1), "norm_type"),
+    (lambda t: ops.grad_norm(t, norm_type=-math.inf), "norm_type"),
+    (lambda t: ops.clip_grads(t, -1.0), "max_norm"),
+    (lambda t: ops.clip_grads(t, math.nan), "max_norm"),
+    (lambda t: ops.clip_grads(t, 1.0, total=z(1)), "grad_total"),
+    (lambda t: ops.clip_grads(t, 1.0, out=[]), "when it is built"),
+])
+def test_wrappers_refuse(call, what):
+    with pytest.raises(_lib.NiwError, match=what):
+        call(ops.TensorTable([]))
+
+
+def group(**kw):
+    g = dict(params=[z(4)], grads=[z(4)], exp_avg=[z(4)], exp_avg_sq=[z(4)])
+    g.update(kw)
+    return g
+
+
+@pytest.mark.parametrize("groups,what", [
+    ([], "1..8 groups"), ([group()] * 9, "1..8 groups"),
+    ([group(lr=[1.0])], "unknown keys"), ([group(grads=None)], "needs params"), ([group(grads=[])], "differ in length"),
+    ([group(exp_avg=[z(4, dtype=torch.bfloat16)])], "expected float32"), ([group(params=[z(4, dtype=torch.bfloat16)])], "master copy"),
+    ([group(master=[z(4)])], "has none"), ([group(grads=[z(2, 2)])], "same order"),
+    ([group(params=[z(2, 3)], grads=[z(3, 2).t()], exp_avg=[z(2, 3)], exp_avg_sq=[z(2, 3)])], "same order"),
+    ([group(params=[z(8)[::2]])], "gaps"), ([group()], "expected CUDA/HIP"), ([group(grads=[z(4, dtype=torch.float64)])], "float64"),
+])
+def test_adam_table_refuses(groups, what):
+    with pytest.raises(_lib.NiwError, match=what):
+        ops.AdamTable(groups)
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(lr=[1e-3, 1e-3]), "lr: 2 values for 1 groups"), (dict(step=[]), "step: 0 values"), (dict(weight_decay=[0.1] * 3), "weight_decay: 3"),
+    (dict(skip_nonfinite=True), "go with max_norm"), (dict(total=z(1, dtype=torch.float64)), "go with max_norm"), (dict(max_norm=-2.0), "max_norm"),
+    (dict(max_norm=1.0, norm_type=3), "norm_type"), (dict(hyper_dev=z(2)), "float32 CUDA"), (dict(max_norm=1.0, total=z(1)), "grad_total"),
+])
+def test_adam_step_tensors_refuses(kw, what):
+    empty = ops.AdamTable([dict(params=[], grads=[], exp_avg=[], exp_avg_sq=[])])
+    with pytest.raises(_lib.NiwError, match=what):
+        ops.adam_step_tensors(empty, **{**dict(lr=1e-3, step=1), **kw})
