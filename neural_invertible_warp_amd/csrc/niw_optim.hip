@@ -18,6 +18,7 @@
 #include "niw_bf16.h"
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -68,16 +69,57 @@ __device__ __forceinline__ int slot_of(const T& t, int c) {
 }
 
 // ------------------------------------------------------------------------------------------------ elements
-__device__ __forceinline__ float load_as_float(const void* p, long long i, int dtype) {
-    if (dtype == NIW_F32) return static_cast<const float*>(p)[i];
-    if (dtype == NIW_BF16) return __builtin_bit_cast(float, (unsigned)static_cast<const unsigned short*>(p)[i] << 16);
-    return (float)static_cast<const _Float16*>(p)[i];
+// Vectors of four elements (16 bytes of fp32, 8 of the half types) that may begin on any element: the aligned(..) attributes promise the
+// compiler no more than that, and gfx950 takes such accesses as one instruction.
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+template <int DT>
+__device__ __forceinline__ float widen(unsigned short bits) {
+    if constexpr (DT == NIW_BF16) return __builtin_bit_cast(float, (unsigned)bits << 16);
+    else return (float)__builtin_bit_cast(_Float16, bits);
+}
+template <int DT>
+__device__ __forceinline__ float load1(const void* p, long long i) {
+    if constexpr (DT == NIW_F32) return static_cast<const float*>(p)[i];
+    else return widen<DT>(static_cast<const unsigned short*>(p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ f32x4 load4(const void* p, long long i) {
+    if constexpr (DT == NIW_F32) return *reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + i);
+    else {
+        const u32x2 w = *reinterpret_cast<const u32x2_any*>(static_cast<const unsigned short*>(p) + i);
+        return f32x4{widen<DT>((unsigned short)w[0]), widen<DT>((unsigned short)(w[0] >> 16)), widen<DT>((unsigned short)w[1]), widen<DT>((unsigned short)(w[1] >> 16))};
+    }
 }
 // rounds to nearest even: bf16 keeps 8 significand bits, fp16 11 (and overflows to infinity above 65504)
-__device__ __forceinline__ void store_from_float(void* p, long long i, int dtype, float x) {
-    if (dtype == NIW_F32) static_cast<float*>(p)[i] = x;
-    else if (dtype == NIW_BF16) static_cast<unsigned short*>(p)[i] = (unsigned short)niw::pack_bf16(x, x);
-    else static_cast<_Float16*>(p)[i] = (_Float16)x;
+template <int DT>
+__device__ __forceinline__ unsigned narrow2(float a, float b) {
+    if constexpr (DT == NIW_BF16) return niw::pack_bf16(a, b);
+    // the fp32 values as they are: without this the compiler folds the multiply-add that made them into v_fma_mixlo_f16, which rounds
+    // once to fp16 -- a parameter would then not be its master copy rounded
+    asm("" : "+v"(a), "+v"(b));
+    return (unsigned)__builtin_bit_cast(unsigned short, (_Float16)a) | (unsigned)__builtin_bit_cast(unsigned short, (_Float16)b) << 16;
+}
+template <int DT>
+__device__ __forceinline__ void store1(void* p, long long i, float x) {
+    if constexpr (DT == NIW_F32) static_cast<float*>(p)[i] = x;
+    else static_cast<unsigned short*>(p)[i] = (unsigned short)narrow2<DT>(x, 0.f);
+}
+template <int DT>
+__device__ __forceinline__ void store4(void* p, long long i, f32x4 x) {
+    if constexpr (DT == NIW_F32) *reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + i) = x;
+    else *reinterpret_cast<u32x2_any*>(static_cast<unsigned short*>(p) + i) = u32x2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])};
+}
+// f(std::integral_constant dtype) for the dtype of a descriptor: the branch is the same for a whole workgroup
+template <class F>
+__device__ __forceinline__ void with_dtype(int dtype, F f) {
+    if (dtype == NIW_F32) f(std::integral_constant<int, NIW_F32>{});
+    else if (dtype == NIW_BF16) f(std::integral_constant<int, NIW_BF16>{});
+    else f(std::integral_constant<int, NIW_F16>{});
 }
 
 // ------------------------------------------------------------------------------------------------ reductions
@@ -99,20 +141,53 @@ __device__ __forceinline__ double block_total(double x) {
     return x;
 }
 
+// what one thread has seen: four running sums (the fp64 units want more than one chain), or the largest bit pattern
+template <int KIND>
+struct Seen {
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    unsigned top = 0;
+    __device__ __forceinline__ void operator()(int k, float x) {
+        if constexpr (KIND == NIW_NORM_2) sum[k & 3] = fma((double)x, (double)x, sum[k & 3]);
+        else top = max(top, __builtin_bit_cast(unsigned, x) & 0x7fffffffu);
+    }
+    __device__ __forceinline__ double total() const {
+        if constexpr (KIND == NIW_NORM_2) return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        else return (double)__builtin_bit_cast(float, top);
+    }
+};
+template <int KIND, int DT>
+__device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, long long begin, long long end) {
+    constexpr int V = DT == NIW_F32 ? 4 : 8, U = 4;      // 16 bytes per thread and load, U loads under way
+    const int tid = threadIdx.x;
+    auto words = [&](long long i) { return *reinterpret_cast<const u32x4_any*>(static_cast<const char*>(p) + i * (16 / V)); };
+    auto take = [&](u32x4 w) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned bits = w[k];          // (a copy: clang's bit_cast of a vector element in place reads element 0)
+            if constexpr (DT == NIW_F32) seen(k, __builtin_bit_cast(float, bits));
+            else { seen(2 * k, widen<DT>((unsigned short)bits)); seen(2 * k + 1, widen<DT>((unsigned short)(bits >> 16))); }
+        }
+    };
+    long long i = begin;
+    for (; i + (long long)kThreads * V * U <= end; i += (long long)kThreads * V * U) {
+        u32x4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = words(i + (u * kThreads + tid) * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u) take(w[u]);
+    }
+    for (i += tid * V; i + V <= end; i += kThreads * V) take(words(i));
+    if (i < end)
+        for (; i < end; ++i) seen(0, load1<DT>(p, i));
+}
+
 template <int KIND>
 __global__ __launch_bounds__(kThreads) void partial_kernel(GradTable t, double* __restrict__ partial) {
     const GradSlot& s = t.s[slot_of(t, blockIdx.x)];
     const long long begin = (long long)((int)blockIdx.x - s.first) * kChunk, end = begin + kChunk < s.n ? begin + kChunk : s.n;
-    const int dtype = s.types & 255;
-    double sum = 0.0;
-    unsigned top = 0;
-    for (long long i = begin + threadIdx.x; i < end; i += kThreads) {
-        const float x = load_as_float(s.g, i, dtype);
-        if constexpr (KIND == NIW_NORM_2) sum = fma((double)x, (double)x, sum);
-        else top = max(top, __builtin_bit_cast(unsigned, x) & 0x7fffffffu);
-    }
-    if constexpr (KIND == NIW_NORM_MAX) sum = (double)__builtin_bit_cast(float, top);
-    sum = block_total<KIND>(sum);
+    Seen<KIND> seen;
+    with_dtype(s.types & 255, [&](auto dt) { see<KIND, decltype(dt)::value>(seen, s.g, begin, end); });
+    const double sum = block_total<KIND>(seen.total());
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
@@ -143,8 +218,22 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(GradTable t, const doubl
     const GradSlot& s = t.s[slot_of(t, blockIdx.x)];
     if (c == 1.f && s.o == s.g) return;
     const long long begin = (long long)((int)blockIdx.x - s.first) * kChunk, end = begin + kChunk < s.n ? begin + kChunk : s.n;
-    for (long long i = begin + threadIdx.x; i < end; i += kThreads)
-        store_from_float(s.o, i, s.types >> 8, c * load_as_float(s.g, i, s.types & 255));
+    with_dtype(s.types & 255, [&](auto gt) {
+        with_dtype(s.types >> 8, [&](auto ot) {
+            constexpr int G = decltype(gt)::value, O = decltype(ot)::value, U = 4;
+            long long i = begin;
+            for (; i + kThreads * 4 * U <= end; i += kThreads * 4 * U) {
+                f32x4 x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) x[u] = load4<G>(s.g, i + (u * kThreads + (int)threadIdx.x) * 4);
+#pragma unroll
+                for (int u = 0; u < U; ++u) store4<O>(s.o, i + (u * kThreads + (int)threadIdx.x) * 4, c * x[u]);
+            }
+            for (i += (int)threadIdx.x * 4; i + 4 <= end; i += kThreads * 4) store4<O>(s.o, i, c * load4<G>(s.g, i));
+            if (i < end)
+                for (; i < end; ++i) store1<O>(s.o, i, c * load1<G>(s.g, i));
+        });
+    });
 }
 
 __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(AdamTable t, const float* __restrict__ hyper_dev, const float* __restrict__ decay_dev,
@@ -165,14 +254,36 @@ __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(AdamTable t, con
     if (decay_dev) decay = decay_dev[k];
     const long long begin = (long long)((int)blockIdx.x - s.first) * kChunk, end = begin + kChunk < s.n ? begin + kChunk : s.n;
     float* const w = s.w ? s.w : static_cast<float*>(s.p);
-    for (long long i = begin + threadIdx.x; i < end; i += kThreads) {
-        float p = w[i], m = s.m[i], v = s.v[i];
-        const float g = niw::mul_rn(c, load_as_float(s.g, i, grad_dtype));
+    auto update = [&](float& p, float g, float& m, float& v) {
         p = fmaf(-decay, p, p);
-        niw::adam_update(p, g, m, v, t.w1, t.b2, t.w2, t.eps, step_size, bc2_sqrt);
-        w[i] = p; s.m[i] = m; s.v[i] = v;
-        if (s.w) store_from_float(s.p, i, param_dtype, p);
-    }
+        niw::adam_update(p, niw::mul_rn(c, g), m, v, t.w1, t.b2, t.w2, t.eps, step_size, bc2_sqrt);
+    };
+    with_dtype(grad_dtype, [&](auto gt) {
+        with_dtype(param_dtype, [&](auto pt) {
+            constexpr int G = decltype(gt)::value, P = decltype(pt)::value;
+            long long i = begin + (int)threadIdx.x * 4;
+            for (; i + 4 <= end; i += kThreads * 4) {
+                f32x4 p = load4<NIW_F32>(w, i), m = load4<NIW_F32>(s.m, i), v = load4<NIW_F32>(s.v, i);
+                const f32x4 g = load4<G>(s.g, i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float pk = p[k], mk = m[k], vk = v[k];
+                    update(pk, g[k], mk, vk);
+                    p[k] = pk; m[k] = mk; v[k] = vk;
+                }
+                store4<NIW_F32>(w, i, p);
+                store4<NIW_F32>(s.m, i, m);
+                store4<NIW_F32>(s.v, i, v);
+                if constexpr (P != NIW_F32) store4<P>(s.p, i, p);
+            }
+            for (; i < end; ++i) {
+                float p = w[i], m = s.m[i], v = s.v[i];
+                update(p, load1<G>(s.g, i), m, v);
+                w[i] = p; s.m[i] = m; s.v[i] = v;
+                if constexpr (P != NIW_F32) store1<P>(s.p, i, p);
+            }
+        });
+    });
 }
 
 // ------------------------------------------------------------------------------------------------ host
