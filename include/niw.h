@@ -385,36 +385,49 @@ int niw_adam_step_multi(const niw_adam_group* groups, int n_groups, double beta1
 
 /* ------------------------------------------------------------------ gradient norm, clipping and Adam over many tensors
  * The optimiser's end of a training step for a LIST of tensors (a module's parameters and their gradients) instead of flat buffers.
- * Lists are HOST arrays of descriptors, read during the call (they travel to the kernels by value: nothing is uploaded, nothing has
- * to outlive the call, a captured graph keeps its own copy); the pointers in them are device pointers.  A list may be empty, and so
- * may every tensor in it.  Data has to be aligned to its own element only.  Everything is stream-ordered, nothing synchronises;
- * results do not depend on how many workgroups run at a time (no float atomics). */
+ * A list is described once: niw_grad_table / niw_adam_table check HOST arrays of descriptors (whose pointers are device pointers) and
+ * turn them into a HOST image, niw_table_store puts the image into device memory of the caller's, and any number of calls then take the
+ * small HOST struct niw_table.  The image is only read by them: one table may serve several streams, threads and captured graphs at a
+ * time (each call its own workspace) as long as the image and the tensors stay where they are.
+ * A list may be empty, and so may every tensor in it; data has to be aligned to its own element only.  Results do not depend on how
+ * many workgroups run at a time (no float atomics). */
 enum niw_dtype { NIW_F32 = 0, NIW_BF16 = 1, NIW_F16 = 2 };
 enum niw_norm_kind { NIW_NORM_2 = 0, NIW_NORM_MAX = 1 };
 
 typedef struct niw_grad_tensor {
     const void* grad;           /* device, n elements of `dtype` */
-    void* out;                  /* device, niw_grad_clip: n elements of `out_dtype` (= grad and its type: in place); niw_grad_norm: unused */
+    void* out;                  /* device, for clipping: n elements of `out_dtype` (= grad and its type: in place); else unused */
     int64_t n;
     int32_t dtype, out_dtype;   /* enum niw_dtype */
 } niw_grad_tensor;
 
-/* NIW_OK, or NIW_ERR_INVALID_ARG for a list that niw_grad_norm (for_clip = 0) / niw_grad_clip (for_clip != 0) must not be given: a null
- * or misaligned pointer, a type or length out of range, and -- for clipping -- an output that overlaps another output, or a gradient
- * other than its own in place.  Host arithmetic only; the two calls below repeat all of it but the overlaps, which are the caller's. */
-int niw_grad_check(const niw_grad_tensor* tensors, int64_t n_tensors, int for_clip);
-/* doubles of the workspace of the two calls below (contents need not survive between calls) */
-int64_t niw_grad_workspace_doubles(const niw_grad_tensor* tensors, int64_t n_tensors);
+typedef struct niw_table {      /* HOST; everything but `image` is filled by niw_grad_table / niw_adam_table and opaque */
+    const void* image;          /* device, 16-byte aligned: set by the caller to where the image was stored */
+    int64_t bytes;              /* of the image */
+    int32_t form, slots, chunks, chunk, groups, wide;
+    int64_t read, moved;
+} niw_table;
+
+/* bytes that hold the image of any list of n tensors */
+int64_t niw_table_bytes(int64_t n_tensors);
+/* image [niw_table_bytes(n_tensors)] HOST, overwritten; table: HOST, filled (image = NULL).  for_clip = 0: a table for niw_grad_norm; != 0: also for
+ * niw_grad_clip, whose outputs must overlap neither each other nor a gradient (their own, in place, excepted).  Host arithmetic only. */
+int niw_grad_table(const niw_grad_tensor* tensors, int64_t n_tensors, int for_clip, void* image, niw_table* table);
+/* dst (device, `bytes` of the table) = the HOST image, which travels inside kernel arguments: stream-ordered, nothing of the host's has to
+ * outlive the call, capturable. */
+int niw_table_store(const void* image, int64_t bytes, void* dst, niw_stream_t stream);
+
+/* doubles of the workspace of a call below (contents need not survive between calls) */
+#define NIW_NORM_WORKSPACE_DOUBLES 1025
 /* total[0] (double, or NULL) = sum of squares of all elements (NIW_NORM_2) or the largest magnitude (NIW_NORM_MAX), and norm[0] (float, or
  * NULL) = its square root / itself.  Squares are formed and summed in double (exact products, no overflow for any fp32 value) in a
  * fixed order; a NaN anywhere gives NaN.  Ranks that hold different shares add (NIW_NORM_2) or take the maximum of their totals. */
-int niw_grad_norm(const niw_grad_tensor* tensors, int64_t n_tensors, int kind, double* workspace, double* total, float* norm, niw_stream_t stream);
+int niw_grad_norm(const niw_table* table, int kind, double* workspace, double* total, float* norm, niw_stream_t stream);
 /* out = c * grad, c = min(1, max_norm / (norm + 1e-6)) formed in double and rounded to fp32 once; the product is formed in fp32 and rounded to
  * out_dtype.  norm: that of the list, or of `total` (device, one double as niw_grad_norm leaves it) when given; norm_out[0] (float) receives it
  * or NULL.  In place with c = 1 nothing is written.  max_norm >= 0; infinity never clips (c = 1).  A norm that is not finite follows the
  * formula: infinite -> c = 0 (finite gradients become 0, infinite ones NaN), NaN -> every gradient NaN. */
-int niw_grad_clip(const niw_grad_tensor* tensors, int64_t n_tensors, int kind, double max_norm, const double* total, double* workspace,
-                  float* norm_out, niw_stream_t stream);
+int niw_grad_clip(const niw_table* table, int kind, double max_norm, const double* total, double* workspace, float* norm_out, niw_stream_t stream);
 
 /* Adam with decoupled weight decay over a list of tensors, under an optional clip by the global norm of its gradients: per element
  *     g = c * grad;  p -= lr * weight_decay * p;  then niw_adam_step's update of p, exp_avg, exp_avg_sq by g
@@ -442,15 +455,16 @@ typedef struct niw_adam_clip {      /* HOST */
     int32_t kind;               /* enum niw_norm_kind */
     int32_t skip_nonfinite;     /* != 0: a norm that is not finite leaves parameters, moments and master copies as they were */
     const double* total;        /* as in niw_grad_clip, or NULL: the norm of the list's gradients */
-    double* workspace;          /* niw_adam_workspace_doubles() doubles */
+    double* workspace;          /* NIW_NORM_WORKSPACE_DOUBLES doubles (may be NULL with `total`) */
     float* norm;                /* [1] receives the norm, or NULL */
 } niw_adam_clip;
-int niw_adam_check(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups);
-int64_t niw_adam_workspace_doubles(const niw_adam_tensor* tensors, int64_t n_tensors);
-/* hyper_dev: DEVICE array [n_groups][2] as in niw_adam_step_multi or NULL; decay_dev: DEVICE array [n_groups] of lr * weight_decay or NULL: both
- * replace what is formed from `hyper` and are read at run time (HIP-graph replays).  clip: NULL = the gradients as they are. */
-int niw_adam_step_tensors(const niw_adam_tensor* tensors, int64_t n_tensors, const niw_adam_hyper* hyper, int n_groups, double beta1, double beta2,
-                          double eps, const float* hyper_dev, const float* decay_dev, const niw_adam_clip* clip, niw_stream_t stream);
+/* as niw_grad_table; what is written (param, exp_avg, exp_avg_sq, master) must overlap nothing else of the list */
+int niw_adam_table(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups, void* image, niw_table* table);
+/* hyper: HOST, one entry per group of the table.  hyper_dev: DEVICE array [n_groups][2] as in niw_adam_step_multi or NULL; decay_dev: DEVICE array
+ * [n_groups] of lr * weight_decay or NULL: both replace what is formed from `hyper` and are read at run time (HIP-graph replays).
+ * clip: NULL = the gradients as they are. */
+int niw_adam_step_tensors(const niw_table* table, const niw_adam_hyper* hyper, double beta1, double beta2, double eps, const float* hyper_dev,
+                          const float* decay_dev, const niw_adam_clip* clip, niw_stream_t stream);
 
 /* ------------------------------------------------------------------ one INN train iteration, forward and backward, one call
  * The body of the reference's train step between zero_grad and the optimizers (model/nerf_inn_llff.py:493-573 Graph.forward +

@@ -35,6 +35,12 @@ class GradTensor(ctypes.Structure):
     _fields_ = [("grad", _vp), ("out", _vp), ("n", _i64), ("dtype", _i32), ("out_dtype", _i32)]
 
 
+class Table(ctypes.Structure):
+    """niw_table of include/niw.h"""
+    _fields_ = [("image", _vp), ("bytes", _i64), ("form", _i32), ("slots", _i32), ("chunks", _i32), ("chunk", _i32), ("groups", _i32), ("wide", _i32),
+                ("read", _i64), ("moved", _i64)]
+
+
 class AdamTensor(ctypes.Structure):
     """niw_adam_tensor of include/niw.h"""
     _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("master", _vp), ("n", _i64), ("param_dtype", _i32),
@@ -118,13 +124,13 @@ SIGNATURES = {
     "niw_render_fwd": (_i, [ctypes.POINTER(RenderDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "niw_adam_step": (_i, [_vp, _vp, _vp, _vp, _i64, _d, _d, _d, _d, _i, _vp, _vp]),
     "niw_adam_step_multi": (_i, [ctypes.POINTER(AdamGroup), _i, _d, _d, _d, _vp, _vp]),
-    "niw_grad_check": (_i, [_vp, _i64, _i]),
-    "niw_grad_workspace_doubles": (_i64, [_vp, _i64]),
-    "niw_grad_norm": (_i, [_vp, _i64, _i, _vp, _vp, _vp, _vp]),
-    "niw_grad_clip": (_i, [_vp, _i64, _i, _d, _vp, _vp, _vp, _vp]),
-    "niw_adam_check": (_i, [_vp, _i64, _i]),
-    "niw_adam_workspace_doubles": (_i64, [_vp, _i64]),
-    "niw_adam_step_tensors": (_i, [_vp, _i64, _vp, _i, _d, _d, _d, _vp, _vp, _vp, _vp]),
+    "niw_table_bytes": (_i64, [_i64]),
+    "niw_grad_table": (_i, [_vp, _i64, _i, _vp, _vp]),
+    "niw_table_store": (_i, [_vp, _i64, _vp, _vp]),
+    "niw_grad_norm": (_i, [_vp, _i, _vp, _vp, _vp, _vp]),
+    "niw_grad_clip": (_i, [_vp, _i, _d, _vp, _vp, _vp, _vp]),
+    "niw_adam_table": (_i, [_vp, _i64, _i, _vp, _vp]),
+    "niw_adam_step_tensors": (_i, [_vp, _vp, _d, _d, _d, _vp, _vp, _vp, _vp]),
     "niw_train_step_prepare": (_i, []),
     "niw_train_step_workspace_floats": (_i64, [ctypes.POINTER(TrainDesc)]),
     "niw_train_step": (_i, [ctypes.POINTER(TrainDesc), _vp, _i, _i, _vp]),

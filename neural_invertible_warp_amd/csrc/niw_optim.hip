@@ -6,9 +6,9 @@
 //
 // All are streams of memory: 2 flops per element for the norm, 3 for clipping, about 18 for Adam.
 //
-// The list goes to the kernels BY VALUE, as many tensors per launch as 4 KB of kernel arguments hold (struct Table): no upload, no
-// device table whose lifetime or stream somebody has to watch, and a captured graph carries its own copy.  A workgroup finds the
-// tensor of its chunk by bisection over the chunks in front of each tensor (scalar loads of the argument segment).
+// The list lies in device memory (the image: one slot per tensor that has elements), so a call is one launch over all tensors, however
+// many.  Tensors are cut into chunks, a workgroup handles whole chunks, and finds the tensor of a chunk by a search that looks at 64
+// tensors at a time (find_slot).
 //
 // Sums.  A square of two 24-bit significands has 48 bits: it is exact in double, and so is its exponent for every fp32 value, so the
 // sum of squares neither overflows (an fp32 sum does from |g| = 1.8e19) nor loses small gradients.  One fp64 fused multiply-add per
@@ -17,6 +17,7 @@
 #include "niw_common.h"
 #include "niw_bf16.h"
 #include <math.h>
+#include <string.h>
 #include <algorithm>
 #include <type_traits>
 #include <vector>
@@ -24,15 +25,38 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 16384;                 // elements of one tensor that one workgroup handles
 constexpr double kClipEps = 1e-6;
 
-// ------------------------------------------------------------------------------------------------ tables
+// Chunks: 16,384 elements, or 4,096 for lists of less than 16 M elements, whose few large chunks would leave compute units idle (a
+// trainer's 1.2 M: clip 17 -> 15 us, of 1000 vectors alike with either).
+constexpr int kChunk = 16384, kSmallChunk = 4096;
+constexpr long long kSmallList = 1024ll * kChunk;
+// The norm runs on at most kNormBlocks workgroups, four per compute unit, that walk the list with its whole width: 1 GB and up read at
+// 7.0 TB/s with 1024, 6.7 with 2048 or 4096, 6.8 with 512 (which costs half-precision lists a quarter: their conversions want more waves).
+constexpr int kNormBlocks = 1024;
+static_assert(kNormBlocks <= NIW_NORM_WORKSPACE_DOUBLES - 1, "a partial sum per workgroup, behind the total");
+// What a clip or an update writes is written by one workgroup per part of a chunk instead: parts of kPart elements in the order of the
+// list keep the pages under way at a time few, which the memory rewards (Adam of 335 M bf16 parameters: parts of 1024 elements 1.70 ms,
+// of 2048 1.74, of 4096 1.76; the norm's fixed workgroups 2.0 to 2.1; the next part's loads issued before this one's stores 1.75).
+// Smaller parts than these reach the rate at which workgroups start.
+constexpr int kAdamPart = 1024;
+constexpr int kClipPart = 4096, kClipPartWide = 2048;      // (wide: fp32 to fp32, 8 bytes per element; in place 933 us against 963 for 2 GB,
+                                                           // but bf16 to fp32 461 against 423 for 335 M)
+// The workgroups of a clip or an update join the norm's partial sums themselves as long as they are few (kFoldGrid): saves a launch,
+// 3 us of the trainer's 18; with 120,000 workgroups one more launch is cheaper (2 GB in place: 963 us against 973).
+constexpr int kFoldGrid = 4096;
+// Lists that move more than the 256 MB of memory-side cache hold go past the caches (non-temporal); a norm still leaves the last
+// kCache bytes of gradients in it, which the clip or update behind it reads first: it walks the list backwards.
+constexpr int64_t kCache = 192ll << 20;
+
+
+// ------------------------------------------------------------------------------------------------ the image of a list
+enum Form { kFormNorm = 1, kFormClip = 2, kFormAdam = 3 };
 struct GradSlot {
     const void* g;
     void* o;
     long long n;
-    int first;                                // chunks of the tensors in front of this one in the launch
+    int first;                                // chunks of the tensors in front of this one
     int types;                                // dtype | out_dtype << 8
 };
 struct AdamSlot {
@@ -43,29 +67,87 @@ struct AdamSlot {
     float* w;                                 // master copy or null
     long long n;
     int first;
-    int types;                                // param_dtype | grad_dtype << 8 | group << 16
+    int types;                                // grad_dtype | param_dtype << 8 | group << 16
+    long long pad;
 };
-template <class Slot, int N>
-struct Table {
-    Slot s[N];
-    int count, chunks;
-};
-using GradTable = Table<GradSlot, 120>;
-struct AdamTable : Table<AdamSlot, 64> {
-    float step_size[NIW_ADAM_MAX_GROUPS], bc2_sqrt[NIW_ADAM_MAX_GROUPS], decay[NIW_ADAM_MAX_GROUPS];
-    float w1, b2, w2, eps;
-};
-static_assert(sizeof(GradTable) <= 4000 && sizeof(AdamTable) <= 4000, "kernel arguments are limited to 4 KB");
+static_assert(sizeof(GradSlot) == 32 && sizeof(AdamSlot) == 64, "slots are read as 16-byte pieces");
 
-// the tensor that chunk c of the launch belongs to
-template <class T>
-__device__ __forceinline__ int slot_of(const T& t, int c) {
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.s[mid].first <= c) lo = mid; else hi = mid - 1;
+// device side of a table: the slots, then `first` of every slot again as an array of its own for the search
+template <class Slot>
+struct List {
+    const Slot* slots;
+    int count, chunks, chunk;
+    __device__ const int* first() const { return reinterpret_cast<const int*>(slots + count); }
+};
+
+// The tensor that chunk c belongs to: every lane looks at one of 64 evenly spaced tensors and the vote of the wave narrows the list to
+// the stretch behind the last that begins at or before c -- two dependent loads for up to 4096 tensors, where a bisection takes twelve.
+__device__ __forceinline__ int find_slot(const int* first, int count, int c) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = count;
+    while (n > 1) {
+        const int stride = (n + 63) >> 6, at = lane * stride;
+        const int v = at < n ? first[lo + at] : 0x7fffffff;
+        const int k = __popcll(__ballot(v <= c)) - 1;
+        lo += k * stride;
+        n = min(stride, n - k * stride);
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// A tensor's first chunk begins with its `head`: the elements in front of the first 128-byte boundary of the stream that matters most (the
+// one that is written, or the only one that is read).  Everything behind it is walked in whole cache lines of that stream, and of the
+// others where they have the same offset, as they have in buckets.
+constexpr int kLine = 128;
+__host__ __device__ inline int head_of(const void* p, int size, long long n) {
+    const int head = (int)((0 - reinterpret_cast<uintptr_t>(p)) & (kLine - 1)) / size;
+    return head < n ? head : (int)n;
+}
+__host__ __device__ inline int size_of(int dtype) { return dtype == NIW_F32 ? 4 : 2; }
+__host__ __device__ inline int head_of(const GradSlot& s, bool written) {
+    return written ? head_of(s.o, size_of(s.types >> 8), s.n) : head_of(s.g, size_of(s.types & 255), s.n);
+}
+__host__ __device__ inline int head_of(const AdamSlot& s, bool written) {
+    return written ? head_of(s.w ? s.w : s.p, 4, s.n) : head_of(s.g, size_of(s.types & 255), s.n);
+}
+// chunks of a tensor: enough for either head
+template <class Slot>
+__host__ __device__ inline long long chunks_of(const Slot& s, int chunk) {
+    return (s.n + chunk - 1) / chunk;
+}
+
+// f(slot, chunk, head, begin, end) for the chunks of this workgroup (the norm: a fixed number of workgroups)
+template <class Slot, class F>
+__device__ __forceinline__ void for_chunks(const List<Slot>& list, F f) {
+    int lo = 0, hi = 0, head = 0;             // chunks of the slot at hand
+    Slot s{};
+    for (int c = blockIdx.x; c < list.chunks; c += gridDim.x) {
+        if (c < lo || c >= hi) {
+            s = list.slots[find_slot(list.first(), list.count, c)];
+            lo = s.first;
+            hi = lo + (int)chunks_of(s, list.chunk);
+            head = head_of(s, false);
+        }
+        // the first chunk holds the head and a whole chunk behind it; the last one ends early or is empty
+        const long long begin = c == lo ? 0 : head + (long long)(c - lo) * list.chunk, end = head + (long long)(c - lo + 1) * list.chunk;
+        if (begin < s.n) f(s, c, begin == 0 ? head : 0, begin, end < s.n ? end : s.n);
+    }
+}
+// parts of at most `part` elements that a chunk is cut into
+template <class Slot>
+__host__ __device__ inline int parts_of(const List<Slot>& list, int part) {
+    return list.chunk > part ? list.chunk / part : 1;
+}
+// f(slot, head, begin, end) for the part of this workgroup (one workgroup per part), from the list's end backwards
+template <int PART, class Slot, class F>
+__device__ __forceinline__ void for_part(const List<Slot>& list, F f) {
+    const int split = parts_of(list, PART), b = (int)blockIdx.x / split, part = split - 1 - (int)blockIdx.x % split;
+    const int c = list.chunks - 1 - b;
+    if (c < 0) return;
+    const Slot s = list.slots[find_slot(list.first(), list.count, c)];
+    const int head = head_of(s, true), step = list.chunk / split;
+    const long long at = (long long)(c - s.first) * list.chunk + part * step, begin = at == 0 ? 0 : head + at, end = head + at + step;
+    if (begin < s.n) f(s, begin == 0 ? head : 0, begin, end < s.n ? end : s.n);
 }
 
 // ------------------------------------------------------------------------------------------------ elements
@@ -87,11 +169,22 @@ __device__ __forceinline__ float load1(const void* p, long long i) {
     if constexpr (DT == NIW_F32) return static_cast<const float*>(p)[i];
     else return widen<DT>(static_cast<const unsigned short*>(p)[i]);
 }
-template <int DT>
+// NT: past the caches (a list that does not fit them anyway leaves them to what does)
+template <bool NT, class V>
+__device__ __forceinline__ V get(const V* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool NT, class V, class X>
+__device__ __forceinline__ void put(V* p, X x) {
+    if constexpr (NT) __builtin_nontemporal_store((V)x, p);
+    else *p = x;
+}
+template <bool NT, int DT>
 __device__ __forceinline__ f32x4 load4(const void* p, long long i) {
-    if constexpr (DT == NIW_F32) return *reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + i);
+    if constexpr (DT == NIW_F32) return get<NT>(reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + i));
     else {
-        const u32x2 w = *reinterpret_cast<const u32x2_any*>(static_cast<const unsigned short*>(p) + i);
+        const u32x2 w = get<NT>(reinterpret_cast<const u32x2_any*>(static_cast<const unsigned short*>(p) + i));
         return f32x4{widen<DT>((unsigned short)w[0]), widen<DT>((unsigned short)(w[0] >> 16)), widen<DT>((unsigned short)w[1]), widen<DT>((unsigned short)(w[1] >> 16))};
     }
 }
@@ -109,10 +202,10 @@ __device__ __forceinline__ void store1(void* p, long long i, float x) {
     if constexpr (DT == NIW_F32) static_cast<float*>(p)[i] = x;
     else static_cast<unsigned short*>(p)[i] = (unsigned short)narrow2<DT>(x, 0.f);
 }
-template <int DT>
+template <bool NT, int DT>
 __device__ __forceinline__ void store4(void* p, long long i, f32x4 x) {
-    if constexpr (DT == NIW_F32) *reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + i) = x;
-    else *reinterpret_cast<u32x2_any*>(static_cast<unsigned short*>(p) + i) = u32x2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])};
+    if constexpr (DT == NIW_F32) put<NT>(reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + i), x);
+    else put<NT>(reinterpret_cast<u32x2_any*>(static_cast<unsigned short*>(p) + i), u32x2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])});
 }
 // f(std::integral_constant dtype) for the dtype of a descriptor: the branch is the same for a whole workgroup
 template <class F>
@@ -123,7 +216,6 @@ __device__ __forceinline__ void with_dtype(int dtype, F f) {
 }
 
 // ------------------------------------------------------------------------------------------------ reductions
-// accumulators: the sum of squares as a double, the maximum as the integer bits of |g| held in a double's place
 template <int KIND>
 __device__ __forceinline__ double join(double a, double b) {
     if constexpr (KIND == NIW_NORM_2) return a + b;
@@ -131,13 +223,14 @@ __device__ __forceinline__ double join(double a, double b) {
 }
 template <int KIND>
 __device__ __forceinline__ double block_total(double x) {
-    __shared__ double part[16];
+    __shared__ double part[kThreads / 64];
 #pragma unroll
     for (int m = 32; m; m >>= 1) x = join<KIND>(x, __shfl_xor(x, m, 64));
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
     __syncthreads();
     x = part[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) x = join<KIND>(x, part[w]);
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) x = join<KIND>(x, part[w]);
     return x;
 }
 
@@ -155,11 +248,11 @@ struct Seen {
         else return (double)__builtin_bit_cast(float, top);
     }
 };
-template <int KIND, int DT>
-__device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, long long begin, long long end) {
+template <int KIND, int DT, bool NT>
+__device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, int head, long long begin, long long end) {
     constexpr int V = DT == NIW_F32 ? 4 : 8, U = 4;      // 16 bytes per thread and load, U loads under way
     const int tid = threadIdx.x;
-    auto words = [&](long long i) { return *reinterpret_cast<const u32x4_any*>(static_cast<const char*>(p) + i * (16 / V)); };
+    auto words = [&](long long i) { return get<NT>(reinterpret_cast<const u32x4_any*>(static_cast<const char*>(p) + i * (16 / V))); };
     auto take = [&](u32x4 w) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -168,7 +261,8 @@ __device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, long long b
             else { seen(2 * k, widen<DT>((unsigned short)bits)); seen(2 * k + 1, widen<DT>((unsigned short)(bits >> 16))); }
         }
     };
-    long long i = begin;
+    if (tid < head) seen(0, load1<DT>(p, tid));
+    long long i = begin + head;
     for (; i + (long long)kThreads * V * U <= end; i += (long long)kThreads * V * U) {
         u32x4 w[U];
 #pragma unroll
@@ -177,137 +271,156 @@ __device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, long long b
         for (int u = 0; u < U; ++u) take(w[u]);
     }
     for (i += tid * V; i + V <= end; i += kThreads * V) take(words(i));
-    if (i < end)
-        for (; i < end; ++i) seen(0, load1<DT>(p, i));
+    for (; i < end; ++i) seen(0, load1<DT>(p, i));
 }
 
-template <int KIND>
-__global__ __launch_bounds__(kThreads) void partial_kernel(GradTable t, double* __restrict__ partial) {
-    const GradSlot& s = t.s[slot_of(t, blockIdx.x)];
-    const long long begin = (long long)((int)blockIdx.x - s.first) * kChunk, end = begin + kChunk < s.n ? begin + kChunk : s.n;
+// chunks in front of `cached` are read past the caches: what a clip reads again is the end of the list
+template <int KIND, class Slot>
+__global__ __launch_bounds__(kThreads) void partial_kernel(List<Slot> list, int cached, double* __restrict__ partial) {
     Seen<KIND> seen;
-    with_dtype(s.types & 255, [&](auto dt) { see<KIND, decltype(dt)::value>(seen, s.g, begin, end); });
+    for_chunks(list, [&](const Slot& s, int c, int head, long long begin, long long end) {
+        with_dtype(s.types & 255, [&](auto dt) {
+            if (c < cached) see<KIND, decltype(dt)::value, true>(seen, s.g, head, begin, end);
+            else see<KIND, decltype(dt)::value, false>(seen, s.g, head, begin, end);
+        });
+    });
     const double sum = block_total<KIND>(seen.total());
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-__device__ __forceinline__ double norm_of(double total, int kind) { return kind == NIW_NORM_2 ? sqrt(total) : total; }
+// the total of n partial sums, in every thread: the same order wherever it is formed
+template <int KIND>
+__device__ __forceinline__ double total_of(const double* __restrict__ partial, int n) {
+    if (n == 1) return partial[0];
+    double x = 0.0;
+    for (int i = threadIdx.x; i < n; i += kThreads) x = join<KIND>(x, partial[i]);
+    return block_total<KIND>(x);
+}
+template <int KIND>
+__device__ __forceinline__ double norm_of(double total) { return KIND == NIW_NORM_2 ? sqrt(total) : total; }
 
 template <int KIND>
-__global__ __launch_bounds__(1024) void finish_kernel(const double* __restrict__ partial, long long n, double* __restrict__ total, float* __restrict__ norm) {
-    double x = 0.0;
-    for (long long i = threadIdx.x; i < n; i += 1024) x = join<KIND>(x, partial[i]);
-    x = block_total<KIND>(x);
+__global__ __launch_bounds__(kThreads) void finish_kernel(const double* __restrict__ partial, int n, double* __restrict__ total, float* __restrict__ norm) {
+    const double x = n ? total_of<KIND>(partial, n) : 0.0;
     if (threadIdx.x == 0) {
         if (total) total[0] = x;
-        if (norm) norm[0] = (float)norm_of(x, KIND);
+        if (norm) norm[0] = (float)norm_of<KIND>(x);
     }
 }
 
-__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
-    if (isinf(max_norm)) return 1.f;
-    const double c = max_norm / (norm + kClipEps);
-    return c < 1.0 ? (float)c : (c != c ? (float)c : 1.f);
+// what a clip goes by: n_partial sums of the norm's launch (or the one total), joined by every workgroup for itself
+struct Clip {
+    const double* partial;                    // null: no clip
+    float* norm_out;
+    double max_norm;
+    int n_partial, skip_nonfinite;
+};
+// -> the factor; `skip`: leave everything as it is
+template <int KIND>
+__device__ __forceinline__ float clip_factor(const Clip& clip, bool& skip) {
+    skip = false;
+    if (!clip.partial) return 1.f;
+    const double norm = norm_of<KIND>(total_of<KIND>(clip.partial, clip.n_partial));
+    if (clip.norm_out && blockIdx.x == 0 && threadIdx.x == 0) clip.norm_out[0] = (float)norm;
+    skip = clip.skip_nonfinite && !isfinite(norm);
+    if (isinf(clip.max_norm)) return 1.f;
+    const double c = clip.max_norm / (norm + kClipEps);
+    return c < 1.0 || c != c ? (float)c : 1.f;
 }
 
-__global__ __launch_bounds__(kThreads) void clip_kernel(GradTable t, const double* __restrict__ total, int kind, double max_norm, float* __restrict__ norm_out) {
-    const double norm = norm_of(total[0], kind);
-    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
-    if (t.count == 0) return;
-    const float c = clip_factor(norm, max_norm);
-    const GradSlot& s = t.s[slot_of(t, blockIdx.x)];
-    if (c == 1.f && s.o == s.g) return;
-    const long long begin = (long long)((int)blockIdx.x - s.first) * kChunk, end = begin + kChunk < s.n ? begin + kChunk : s.n;
-    with_dtype(s.types & 255, [&](auto gt) {
-        with_dtype(s.types >> 8, [&](auto ot) {
-            constexpr int G = decltype(gt)::value, O = decltype(ot)::value, U = 4;
-            long long i = begin;
-            for (; i + kThreads * 4 * U <= end; i += kThreads * 4 * U) {
-                f32x4 x[U];
+template <int KIND, bool NT, int PART>
+__global__ __launch_bounds__(kThreads) void clip_kernel(List<GradSlot> list, Clip clip) {
+    bool skip;
+    const float c = clip_factor<KIND>(clip, skip);
+    for_part<PART>(list, [&](const GradSlot& s, int head, long long begin, long long end) {
+        if (c == 1.f && s.o == s.g) return;
+        with_dtype(s.types & 255, [&](auto gt) {
+            with_dtype(s.types >> 8, [&](auto ot) {
+                constexpr int G = decltype(gt)::value, O = decltype(ot)::value, U = PART / (kThreads * 4);
+                const int tid = threadIdx.x;
+                if (tid < head) store1<O>(s.o, tid, c * load1<G>(s.g, tid));
+                long long i = begin + head;
+                for (; i + kThreads * 4 * U <= end; i += kThreads * 4 * U) {
+                    f32x4 x[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = load4<G>(s.g, i + (u * kThreads + (int)threadIdx.x) * 4);
+                    for (int u = 0; u < U; ++u) x[u] = load4<NT, G>(s.g, i + (u * kThreads + tid) * 4);
 #pragma unroll
-                for (int u = 0; u < U; ++u) store4<O>(s.o, i + (u * kThreads + (int)threadIdx.x) * 4, c * x[u]);
-            }
-            for (i += (int)threadIdx.x * 4; i + 4 <= end; i += kThreads * 4) store4<O>(s.o, i, c * load4<G>(s.g, i));
-            if (i < end)
-                for (; i < end; ++i) store1<O>(s.o, i, c * load1<G>(s.g, i));
-        });
-    });
-}
-
-__global__ __launch_bounds__(kThreads) void adam_tensors_kernel(AdamTable t, const float* __restrict__ hyper_dev, const float* __restrict__ decay_dev,
-                                                                const double* __restrict__ total, int kind, int skip_nonfinite, double max_norm,
-                                                                float* __restrict__ norm_out) {
-    float c = 1.f;
-    if (total) {
-        const double norm = norm_of(total[0], kind);
-        if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
-        if (skip_nonfinite && !isfinite(norm)) return;
-        c = clip_factor(norm, max_norm);
-    }
-    if (t.count == 0) return;
-    const AdamSlot& s = t.s[slot_of(t, blockIdx.x)];
-    const int param_dtype = s.types & 255, grad_dtype = (s.types >> 8) & 255, k = s.types >> 16;
-    float step_size = t.step_size[k], bc2_sqrt = t.bc2_sqrt[k], decay = t.decay[k];
-    if (hyper_dev) { step_size = hyper_dev[2 * k]; bc2_sqrt = hyper_dev[2 * k + 1]; }
-    if (decay_dev) decay = decay_dev[k];
-    const long long begin = (long long)((int)blockIdx.x - s.first) * kChunk, end = begin + kChunk < s.n ? begin + kChunk : s.n;
-    float* const w = s.w ? s.w : static_cast<float*>(s.p);
-    auto update = [&](float& p, float g, float& m, float& v) {
-        p = fmaf(-decay, p, p);
-        niw::adam_update(p, niw::mul_rn(c, g), m, v, t.w1, t.b2, t.w2, t.eps, step_size, bc2_sqrt);
-    };
-    with_dtype(grad_dtype, [&](auto gt) {
-        with_dtype(param_dtype, [&](auto pt) {
-            constexpr int G = decltype(gt)::value, P = decltype(pt)::value;
-            long long i = begin + (int)threadIdx.x * 4;
-            for (; i + 4 <= end; i += kThreads * 4) {
-                f32x4 p = load4<NIW_F32>(w, i), m = load4<NIW_F32>(s.m, i), v = load4<NIW_F32>(s.v, i);
-                const f32x4 g = load4<G>(s.g, i);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float pk = p[k], mk = m[k], vk = v[k];
-                    update(pk, g[k], mk, vk);
-                    p[k] = pk; m[k] = mk; v[k] = vk;
+                    for (int u = 0; u < U; ++u) store4<NT, O>(s.o, i + (u * kThreads + tid) * 4, c * x[u]);
                 }
-                store4<NIW_F32>(w, i, p);
-                store4<NIW_F32>(s.m, i, m);
-                store4<NIW_F32>(s.v, i, v);
-                if constexpr (P != NIW_F32) store4<P>(s.p, i, p);
-            }
-            for (; i < end; ++i) {
-                float p = w[i], m = s.m[i], v = s.v[i];
-                update(p, load1<G>(s.g, i), m, v);
-                w[i] = p; s.m[i] = m; s.v[i] = v;
-                if constexpr (P != NIW_F32) store1<P>(s.p, i, p);
-            }
+                for (i += tid * 4; i + 4 <= end; i += kThreads * 4) store4<NT, O>(s.o, i, c * load4<NT, G>(s.g, i));
+                for (; i < end; ++i) store1<O>(s.o, i, c * load1<G>(s.g, i));
+            });
         });
     });
+}
+
+struct AdamArgs {
+    float step_size[NIW_ADAM_MAX_GROUPS], bc2_sqrt[NIW_ADAM_MAX_GROUPS], decay[NIW_ADAM_MAX_GROUPS];
+    float w1, b2, w2, eps;
+    const float* hyper_dev;
+    const float* decay_dev;
+};
+
+template <int KIND, bool NT>
+__global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> list, AdamArgs a, Clip clip) {
+    bool skip;
+    const float c = clip_factor<KIND>(clip, skip);
+    if (skip) return;
+    for_part<kAdamPart>(list, [&](const AdamSlot& s, int head, long long begin, long long end) {
+        const int k = __builtin_amdgcn_readfirstlane(s.types >> 16);
+        const float step_size = a.hyper_dev ? a.hyper_dev[2 * k] : a.step_size[k], bc2_sqrt = a.hyper_dev ? a.hyper_dev[2 * k + 1] : a.bc2_sqrt[k];
+        const float decay = a.decay_dev ? a.decay_dev[k] : a.decay[k];
+        float* const w = s.w ? s.w : static_cast<float*>(s.p);
+        auto update = [&](float& p, float g, float& m, float& v) {
+            p = fmaf(-decay, p, p);
+            niw::adam_update(p, niw::mul_rn(c, g), m, v, a.w1, a.b2, a.w2, a.eps, step_size, bc2_sqrt);
+        };
+        with_dtype(s.types & 255, [&](auto gt) {
+            with_dtype((s.types >> 8) & 255, [&](auto pt) {
+                constexpr int G = decltype(gt)::value, P = decltype(pt)::value;
+                auto one = [&](long long i) {
+                    float p = w[i], m = s.m[i], v = s.v[i];
+                    update(p, load1<G>(s.g, i), m, v);
+                    w[i] = p; s.m[i] = m; s.v[i] = v;
+                    if constexpr (P != NIW_F32) store1<P>(s.p, i, p);
+                };
+                const int tid = threadIdx.x;
+                if (tid < head) one(tid);
+                long long i = begin + head + tid * 4;
+                for (; i + 4 <= end; i += kThreads * 4) {
+                    f32x4 p = load4<NT, NIW_F32>(w, i), m = load4<NT, NIW_F32>(s.m, i), v = load4<NT, NIW_F32>(s.v, i);
+                    const f32x4 g = load4<NT, G>(s.g, i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float pj = p[j], mj = m[j], vj = v[j];
+                        update(pj, g[j], mj, vj);
+                        p[j] = pj; m[j] = mj; v[j] = vj;
+                    }
+                    store4<NT, NIW_F32>(w, i, p);
+                    store4<NT, NIW_F32>(s.m, i, m);
+                    store4<NT, NIW_F32>(s.v, i, v);
+                    if constexpr (P != NIW_F32) store4<NT, P>(s.p, i, p);
+                }
+                for (; i < end; ++i) one(i);
+            });
+        });
+    });
+}
+
+// a piece of a host image, by value
+struct Piece {
+    u32x4 d[240];
+};
+__global__ __launch_bounds__(kThreads) void store_kernel(Piece piece, u32x4* __restrict__ dst, int n) {
+    if ((int)threadIdx.x < n) dst[threadIdx.x] = piece.d[threadIdx.x];
 }
 
 // ------------------------------------------------------------------------------------------------ host
-int size_of(int dtype) { return dtype == NIW_F32 ? 4 : 2; }
 bool known(int dtype) { return dtype == NIW_F32 || dtype == NIW_BF16 || dtype == NIW_F16; }
 bool aligned(const void* p, int size) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(size - 1)) == 0; }
-long long chunks_of(long long n) { return (n + kChunk - 1) / kChunk; }
-constexpr int64_t kMaxElements = 1ll << 44;   // (chunks of one tensor stay far below 2^31)
-
-int check_grads(const char* what, const niw_grad_tensor* t, int64_t count, bool for_clip) {
-    NIW_REQUIRE(count >= 0 && (t || count == 0), "%s: %lld tensors at a null pointer", what, (long long)count);
-    for (int64_t i = 0; i < count; ++i) {
-        NIW_REQUIRE(t[i].n >= 0 && t[i].n <= kMaxElements, "%s: tensor %lld has n=%lld", what, (long long)i, (long long)t[i].n);
-        NIW_REQUIRE(known(t[i].dtype), "%s: tensor %lld has unknown dtype %d", what, (long long)i, t[i].dtype);
-        NIW_REQUIRE(t[i].n == 0 || t[i].grad, "%s: null pointer in tensor %lld", what, (long long)i);
-        NIW_REQUIRE(aligned(t[i].grad, size_of(t[i].dtype)), "%s: tensor %lld is not aligned to its elements", what, (long long)i);
-        if (!for_clip) continue;
-        NIW_REQUIRE(known(t[i].out_dtype), "%s: output %lld has unknown dtype %d", what, (long long)i, t[i].out_dtype);
-        NIW_REQUIRE(t[i].n == 0 || t[i].out, "%s: null pointer in output %lld", what, (long long)i);
-        NIW_REQUIRE(aligned(t[i].out, size_of(t[i].out_dtype)), "%s: output %lld is not aligned to its elements", what, (long long)i);
-        NIW_REQUIRE(t[i].n == 0 || t[i].out != t[i].grad || t[i].out_dtype == t[i].dtype, "%s: tensor %lld in place changes its type", what, (long long)i);
-    }
-    return NIW_OK;
-}
+constexpr int64_t kMaxElements = 1ll << 44, kMaxTensors = 1ll << 20;
+constexpr int64_t kMaxChunks = 0x7fffffffll / (kChunk / kAdamPart);      // (workgroups of a launch are counted in 31 bits)
+int64_t padded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // a range of memory that the call writes (or only reads), for the overlap check
 struct Range {
@@ -332,69 +445,29 @@ void add_range(std::vector<Range>& r, const void* p, int64_t n, int size, int64_
     if (n > 0) r.push_back(Range{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + (uintptr_t)n * size, tensor, writes});
 }
 
-// calls f(table, chunks of the launches before it) for the launches that `count` tensors take; tensors without elements are left out
-template <class T, class Item, class Fill, class Launch>
-int for_tables(const Item* items, int64_t count, T& table, Fill fill, Launch launch) {
-    constexpr int kSlots = sizeof(table.s) / sizeof(table.s[0]);
-    long long before = 0;
-    table.count = table.chunks = 0;
+int check_grads(const char* what, const niw_grad_tensor* t, int64_t count, bool for_clip) {
     for (int64_t i = 0; i < count; ++i) {
-        if (items[i].n == 0) continue;
-        const long long chunks = chunks_of(items[i].n);
-        if (table.count == kSlots || table.chunks + chunks > 0x7fffffffll) {
-            const int rc = launch(table, before);
-            if (rc != NIW_OK) return rc;
-            before += table.chunks;
-            table.count = table.chunks = 0;
-        }
-        fill(table.s[table.count], items[i]);
-        table.s[table.count].first = table.chunks;
-        ++table.count;
-        table.chunks += (int)chunks;
+        NIW_REQUIRE(t[i].n >= 0 && t[i].n <= kMaxElements, "%s: tensor %lld has n=%lld", what, (long long)i, (long long)t[i].n);
+        NIW_REQUIRE(known(t[i].dtype), "%s: tensor %lld has unknown dtype %d", what, (long long)i, t[i].dtype);
+        NIW_REQUIRE(t[i].n == 0 || t[i].grad, "%s: null pointer in tensor %lld", what, (long long)i);
+        NIW_REQUIRE(aligned(t[i].grad, size_of(t[i].dtype)), "%s: tensor %lld is not aligned to its elements", what, (long long)i);
+        if (!for_clip) continue;
+        NIW_REQUIRE(known(t[i].out_dtype), "%s: output %lld has unknown dtype %d", what, (long long)i, t[i].out_dtype);
+        NIW_REQUIRE(t[i].n == 0 || t[i].out, "%s: null pointer in output %lld", what, (long long)i);
+        NIW_REQUIRE(aligned(t[i].out, size_of(t[i].out_dtype)), "%s: output %lld is not aligned to its elements", what, (long long)i);
+        NIW_REQUIRE(t[i].n == 0 || t[i].out != t[i].grad || t[i].out_dtype == t[i].dtype, "%s: tensor %lld in place changes its type", what, (long long)i);
     }
-    return table.count ? launch(table, before) : NIW_OK;
-}
-
-// the list's total into `total` (and the norm): partial sums of every launch, then one workgroup over them
-template <class Item, class Fill>
-int total_of(const char* what, const Item* items, int64_t count, Fill fill, int kind, double* workspace, double* total, float* norm, hipStream_t st) {
-    GradTable table{};
-    long long partials = 0;
-    const int rc = for_tables(items, count, table, fill, [&](const GradTable& t, long long before) -> int {
-        if (kind == NIW_NORM_2) partial_kernel<NIW_NORM_2><<<t.chunks, kThreads, 0, st>>>(t, workspace + before);
-        else partial_kernel<NIW_NORM_MAX><<<t.chunks, kThreads, 0, st>>>(t, workspace + before);
-        partials = before + t.chunks;
-        NIW_LAUNCH_CHECK(what);
-        return NIW_OK;
-    });
-    if (rc != NIW_OK) return rc;
-    if (kind == NIW_NORM_2) finish_kernel<NIW_NORM_2><<<1, 1024, 0, st>>>(workspace, partials, total, norm);
-    else finish_kernel<NIW_NORM_MAX><<<1, 1024, 0, st>>>(workspace, partials, total, norm);
-    NIW_LAUNCH_CHECK(what);
-    return NIW_OK;
-}
-
-template <class Item>
-int64_t workspace_doubles(const Item* t, int64_t count) {
-    long long n = 1;                          // the total stands in front of the partial sums
-    for (int64_t i = 0; t && i < count; ++i) n += t[i].n > 0 ? chunks_of(t[i].n) : 0;
-    return n;
-}
-
-void fill_grad(GradSlot& s, const niw_grad_tensor& t) {
-    s.g = t.grad; s.o = t.out; s.n = t.n; s.types = t.dtype | t.out_dtype << 8;
-}
-void fill_adam_grad(GradSlot& s, const niw_adam_tensor& t) {
-    s.g = t.grad; s.o = nullptr; s.n = t.n; s.types = t.grad_dtype;
-}
-void fill_adam(AdamSlot& s, const niw_adam_tensor& t) {
-    s.p = t.param; s.g = t.grad; s.m = t.exp_avg; s.v = t.exp_avg_sq; s.w = t.master; s.n = t.n;
-    s.types = t.param_dtype | t.grad_dtype << 8 | t.group << 16;
+    if (!for_clip) return NIW_OK;
+    std::vector<Range> r;
+    r.reserve(2 * count);
+    for (int64_t i = 0; i < count; ++i) {
+        if (t[i].out != t[i].grad) add_range(r, t[i].grad, t[i].n, size_of(t[i].dtype), i, false);
+        add_range(r, t[i].out, t[i].n, size_of(t[i].out_dtype), i, true);
+    }
+    return check_overlaps(what, r);
 }
 
 int check_adam(const char* what, const niw_adam_tensor* t, int64_t count, int n_groups) {
-    NIW_REQUIRE(count >= 0 && (t || count == 0), "%s: %lld tensors at a null pointer", what, (long long)count);
-    NIW_REQUIRE(n_groups >= 1 && n_groups <= NIW_ADAM_MAX_GROUPS, "%s: 1..%d groups (got %d)", what, NIW_ADAM_MAX_GROUPS, n_groups);
     for (int64_t i = 0; i < count; ++i) {
         const niw_adam_tensor& x = t[i];
         NIW_REQUIRE(x.n >= 0 && x.n <= kMaxElements, "%s: tensor %lld has n=%lld", what, (long long)i, (long long)x.n);
@@ -406,97 +479,192 @@ int check_adam(const char* what, const niw_adam_tensor* t, int64_t count, int n_
         NIW_REQUIRE(aligned(x.param, size_of(x.param_dtype)) && aligned(x.grad, size_of(x.grad_dtype)) && aligned(x.exp_avg, 4) && aligned(x.exp_avg_sq, 4) && aligned(x.master, 4),
                     "%s: tensor %lld is not aligned to its elements", what, (long long)i);
     }
+    std::vector<Range> r;
+    r.reserve(5 * count);
+    for (int64_t i = 0; i < count; ++i) {
+        add_range(r, t[i].param, t[i].n, size_of(t[i].param_dtype), i, true);
+        add_range(r, t[i].grad, t[i].n, size_of(t[i].grad_dtype), i, false);
+        add_range(r, t[i].exp_avg, t[i].n, 4, i, true);
+        add_range(r, t[i].exp_avg_sq, t[i].n, 4, i, true);
+        if (t[i].master) add_range(r, t[i].master, t[i].n, 4, i, true);
+    }
+    return check_overlaps(what, r);
+}
+
+void fill(GradSlot& s, const niw_grad_tensor& t) {
+    s.g = t.grad; s.o = t.out; s.n = t.n; s.types = t.dtype | t.out_dtype << 8;
+}
+void fill(AdamSlot& s, const niw_adam_tensor& t) {
+    s.p = t.param; s.g = t.grad; s.m = t.exp_avg; s.v = t.exp_avg_sq; s.w = t.master; s.n = t.n; s.pad = 0;
+    s.types = t.grad_dtype | t.param_dtype << 8 | t.group << 16;
+}
+
+// bytes of gradients, and bytes that a clip or an update of the tensor moves
+void read_written(const niw_grad_tensor& t, int64_t& read, int64_t& moved) {
+    read += t.n * size_of(t.dtype); moved += t.n * (size_of(t.dtype) + size_of(t.out_dtype));
+}
+void read_written(const niw_adam_tensor& t, int64_t& read, int64_t& moved) {
+    read += t.n * size_of(t.grad_dtype); moved += t.n * (24 + size_of(t.grad_dtype) + (t.master ? 2 : 0));
+}
+
+template <class Slot, class Item>
+int build(const char* what, const Item* items, int64_t count, int form, int groups, void* image, niw_table* table) {
+    long long total = 0;
+    int slots = 0;
+    *table = niw_table{};
+    for (int64_t i = 0; i < count; ++i) {
+        total += items[i].n; slots += items[i].n > 0;
+        read_written(items[i], table->read, table->moved);
+    }
+    table->form = form; table->slots = slots; table->groups = groups;
+    table->chunk = total < kSmallList ? kSmallChunk : kChunk;
+    table->bytes = padded((int64_t)slots * (sizeof(Slot) + sizeof(int)));
+    memset(image, 0, table->bytes);
+    Slot* s = static_cast<Slot*>(image);
+    int* first = reinterpret_cast<int*>(s + slots);
+    long long chunks = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (items[i].n == 0) continue;
+        fill(*s, items[i]);
+        s->first = *first = (int)chunks;
+        chunks += chunks_of(*s, table->chunk);
+        ++s; ++first;
+        NIW_REQUIRE(chunks <= kMaxChunks, "%s: more than %lld chunks of %d elements", what, (long long)kMaxChunks, table->chunk);
+    }
+    table->chunks = (int)chunks;
+    table->wide = table->moved >= 8 * total;
     return NIW_OK;
+}
+
+template <class Slot>
+List<Slot> list_of(const niw_table& t) {
+    return List<Slot>{static_cast<const Slot*>(t.image), t.slots, t.chunks, t.chunk};
+}
+int check_table(const char* what, const niw_table* t, bool form_fits) {
+    NIW_REQUIRE(t, "%s: null pointer", what);
+    NIW_REQUIRE(form_fits, "%s: a table of form %d", what, t->form);
+    NIW_REQUIRE(t->slots == 0 || (t->image && aligned(t->image, 16)), "%s: the table's image is not stored", what);
+    return NIW_OK;
+}
+
+// the launch that leaves the partial sums of the list in `partial`; -> their number
+template <class Slot>
+int launch_partials(const List<Slot>& list, const niw_table& t, int kind, double* partial, hipStream_t st) {
+    const int grid = list.chunks < kNormBlocks ? list.chunks : kNormBlocks;
+    if (grid == 0) return 0;
+    const int cached = t.read <= kCache ? 0 : (int)((double)list.chunks * (1.0 - (double)kCache / (double)t.read));
+    if (kind == NIW_NORM_2) partial_kernel<NIW_NORM_2><<<grid, kThreads, 0, st>>>(list, cached, partial);
+    else partial_kernel<NIW_NORM_MAX><<<grid, kThreads, 0, st>>>(list, cached, partial);
+    return grid;
+}
+void launch_finish(int kind, const double* partial, int n, double* total, float* norm, hipStream_t st) {
+    if (kind == NIW_NORM_2) finish_kernel<NIW_NORM_2><<<1, kThreads, 0, st>>>(partial, n, total, norm);
+    else finish_kernel<NIW_NORM_MAX><<<1, kThreads, 0, st>>>(partial, n, total, norm);
+}
+// one workgroup per part (one for an empty list, whose norm is still written)
+template <class Slot>
+int64_t grid_of(const List<Slot>& list, int part) {
+    return list.chunks < 1 ? 1 : (int64_t)list.chunks * parts_of(list, part);
+}
+// the norm's launches in front of a kernel of `grid` workgroups that clips by it
+template <class Slot>
+void prepare_clip(Clip& clip, const List<Slot>& list, const niw_table& t, int64_t grid, int kind, const double* total, double* workspace, hipStream_t st) {
+    clip.partial = total;
+    clip.n_partial = 1;
+    if (total) return;
+    const int n = launch_partials(list, t, kind, workspace + 1, st);
+    if (n > 0 && grid <= kFoldGrid) { clip.partial = workspace + 1; clip.n_partial = n; return; }
+    launch_finish(kind, workspace + 1, n, workspace, nullptr, st);
+    clip.partial = workspace;
 }
 
 }  // namespace
 
-extern "C" int niw_grad_check(const niw_grad_tensor* tensors, int64_t n_tensors, int for_clip) {
-    const int rc = check_grads("niw_grad_check", tensors, n_tensors, for_clip != 0);
-    if (rc != NIW_OK || !for_clip) return rc;
-    try {
-        std::vector<Range> r;
-        r.reserve(2 * n_tensors);
-        for (int64_t i = 0; i < n_tensors; ++i) {
-            const niw_grad_tensor& t = tensors[i];
-            if (t.out != t.grad) add_range(r, t.grad, t.n, size_of(t.dtype), i, false);
-            add_range(r, t.out, t.n, size_of(t.out_dtype), i, true);
-        }
-        return check_overlaps("niw_grad_check", r);
-    } catch (...) {
-        niw_set_error("niw_grad_check: out of host memory");
-        return NIW_ERR_INVALID_ARG;
-    }
+extern "C" int64_t niw_table_bytes(int64_t n_tensors) { return n_tensors < 0 ? 0 : padded(n_tensors * (int64_t)(sizeof(AdamSlot) + sizeof(int))); }
+
+extern "C" int niw_grad_table(const niw_grad_tensor* tensors, int64_t n_tensors, int for_clip, void* image, niw_table* table) try {
+    NIW_REQUIRE(n_tensors >= 0 && n_tensors <= kMaxTensors && (tensors || n_tensors == 0), "niw_grad_table: %lld tensors at %p", (long long)n_tensors, (const void*)tensors);
+    NIW_REQUIRE(table && (image || n_tensors == 0), "niw_grad_table: null pointer");
+    const int rc = check_grads("niw_grad_table", tensors, n_tensors, for_clip != 0);
+    return rc != NIW_OK ? rc : build<GradSlot>("niw_grad_table", tensors, n_tensors, for_clip ? kFormClip : kFormNorm, 0, image, table);
+} catch (...) {
+    niw_set_error("niw_grad_table: out of host memory");
+    return NIW_ERR_INVALID_ARG;
 }
 
-extern "C" int64_t niw_grad_workspace_doubles(const niw_grad_tensor* tensors, int64_t n_tensors) { return workspace_doubles(tensors, n_tensors); }
+extern "C" int niw_adam_table(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups, void* image, niw_table* table) try {
+    NIW_REQUIRE(n_tensors >= 0 && n_tensors <= kMaxTensors && (tensors || n_tensors == 0), "niw_adam_table: %lld tensors at %p", (long long)n_tensors, (const void*)tensors);
+    NIW_REQUIRE(table && (image || n_tensors == 0), "niw_adam_table: null pointer");
+    NIW_REQUIRE(n_groups >= 1 && n_groups <= NIW_ADAM_MAX_GROUPS, "niw_adam_table: 1..%d groups (got %d)", NIW_ADAM_MAX_GROUPS, n_groups);
+    const int rc = check_adam("niw_adam_table", tensors, n_tensors, n_groups);
+    return rc != NIW_OK ? rc : build<AdamSlot>("niw_adam_table", tensors, n_tensors, kFormAdam, n_groups, image, table);
+} catch (...) {
+    niw_set_error("niw_adam_table: out of host memory");
+    return NIW_ERR_INVALID_ARG;
+}
 
-extern "C" int niw_grad_norm(const niw_grad_tensor* tensors, int64_t n_tensors, int kind, double* workspace, double* total, float* norm, niw_stream_t stream) {
-    const int rc = check_grads("niw_grad_norm", tensors, n_tensors, false);
+extern "C" int niw_table_store(const void* image, int64_t bytes, void* dst, niw_stream_t stream) {
+    NIW_REQUIRE(bytes >= 0 && bytes % 16 == 0, "niw_table_store: %lld bytes", (long long)bytes);
+    NIW_REQUIRE(bytes == 0 || (image && dst && aligned(dst, 16)), "niw_table_store: null or misaligned pointer");
+    for (int64_t at = 0; at < bytes; at += sizeof(Piece)) {
+        const int64_t size = bytes - at < (int64_t)sizeof(Piece) ? bytes - at : (int64_t)sizeof(Piece);
+        Piece piece;
+        memcpy(&piece, static_cast<const char*>(image) + at, size);
+        store_kernel<<<1, kThreads, 0, (hipStream_t)stream>>>(piece, reinterpret_cast<u32x4*>(static_cast<char*>(dst) + at), (int)(size / 16));
+    }
+    NIW_LAUNCH_CHECK("niw_table_store");
+    return NIW_OK;
+}
+
+extern "C" int niw_grad_norm(const niw_table* table, int kind, double* workspace, double* total, float* norm, niw_stream_t stream) {
+    const int rc = check_table("niw_grad_norm", table, table && (table->form == kFormNorm || table->form == kFormClip));
     if (rc != NIW_OK) return rc;
     NIW_REQUIRE(kind == NIW_NORM_2 || kind == NIW_NORM_MAX, "niw_grad_norm: unknown kind %d", kind);
     NIW_REQUIRE(workspace && (total || norm), "niw_grad_norm: null pointer");
-    return total_of("niw_grad_norm", tensors, n_tensors, fill_grad, kind, workspace + 1, total, norm, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    const int n = launch_partials(list_of<GradSlot>(*table), *table, kind, workspace + 1, st);
+    launch_finish(kind, workspace + 1, n, total, norm, st);
+    NIW_LAUNCH_CHECK("niw_grad_norm");
+    return NIW_OK;
 }
 
-extern "C" int niw_grad_clip(const niw_grad_tensor* tensors, int64_t n_tensors, int kind, double max_norm, const double* total, double* workspace,
-                             float* norm_out, niw_stream_t stream) {
-    int rc = check_grads("niw_grad_clip", tensors, n_tensors, true);
+extern "C" int niw_grad_clip(const niw_table* table, int kind, double max_norm, const double* total, double* workspace, float* norm_out, niw_stream_t stream) {
+    const int rc = check_table("niw_grad_clip", table, table && table->form == kFormClip);
     if (rc != NIW_OK) return rc;
     NIW_REQUIRE(kind == NIW_NORM_2 || kind == NIW_NORM_MAX, "niw_grad_clip: unknown kind %d", kind);
     NIW_REQUIRE(max_norm >= 0.0, "niw_grad_clip: max_norm=%g", max_norm);
     NIW_REQUIRE(workspace || total, "niw_grad_clip: null pointer");
     hipStream_t st = (hipStream_t)stream;
-    if (!total) {
-        rc = total_of("niw_grad_clip", tensors, n_tensors, fill_grad, kind, workspace + 1, workspace, nullptr, st);
-        if (rc != NIW_OK) return rc;
-        total = workspace;
-    }
-    GradTable table{};
-    bool launched = false;
-    rc = for_tables(tensors, n_tensors, table, fill_grad, [&](const GradTable& t, long long) -> int {
-        clip_kernel<<<t.chunks, kThreads, 0, st>>>(t, total, kind, max_norm, launched ? nullptr : norm_out);
-        launched = true;
-        NIW_LAUNCH_CHECK("niw_grad_clip");
-        return NIW_OK;
-    });
-    if (rc != NIW_OK || launched || !norm_out) return rc;
-    clip_kernel<<<1, kThreads, 0, st>>>(table, total, kind, max_norm, norm_out);      // (an empty list: the norm alone)
+    const auto list = list_of<GradSlot>(*table);
+    Clip clip{nullptr, norm_out, max_norm, 1, 0};
+    const bool nt = table->moved > kCache, wide = table->wide != 0;
+    const int64_t grid = grid_of(list, wide ? kClipPartWide : kClipPart);
+    prepare_clip(clip, list, *table, grid, kind, total, workspace, st);
+    auto launch = [&](auto nk, auto past, auto part) {
+        clip_kernel<decltype(nk)::value, decltype(past)::value, decltype(part)::value><<<(unsigned)grid, kThreads, 0, st>>>(list, clip);
+    };
+    auto with_part = [&](auto nk, auto past) {
+        if (wide) launch(nk, past, std::integral_constant<int, kClipPartWide>{});
+        else launch(nk, past, std::integral_constant<int, kClipPart>{});
+    };
+    auto with_nt = [&](auto nk) {
+        if (nt) with_part(nk, std::true_type{});
+        else with_part(nk, std::false_type{});
+    };
+    if (kind == NIW_NORM_2) with_nt(std::integral_constant<int, NIW_NORM_2>{});
+    else with_nt(std::integral_constant<int, NIW_NORM_MAX>{});
     NIW_LAUNCH_CHECK("niw_grad_clip");
     return NIW_OK;
 }
 
-extern "C" int niw_adam_check(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups) {
-    const int rc = check_adam("niw_adam_check", tensors, n_tensors, n_groups);
-    if (rc != NIW_OK) return rc;
-    try {
-        std::vector<Range> r;
-        r.reserve(5 * n_tensors);
-        for (int64_t i = 0; i < n_tensors; ++i) {
-            const niw_adam_tensor& t = tensors[i];
-            add_range(r, t.param, t.n, size_of(t.param_dtype), i, true);
-            add_range(r, t.grad, t.n, size_of(t.grad_dtype), i, false);
-            add_range(r, t.exp_avg, t.n, 4, i, true);
-            add_range(r, t.exp_avg_sq, t.n, 4, i, true);
-            if (t.master) add_range(r, t.master, t.n, 4, i, true);
-        }
-        return check_overlaps("niw_adam_check", r);
-    } catch (...) {
-        niw_set_error("niw_adam_check: out of host memory");
-        return NIW_ERR_INVALID_ARG;
-    }
-}
-
-extern "C" int64_t niw_adam_workspace_doubles(const niw_adam_tensor* tensors, int64_t n_tensors) { return workspace_doubles(tensors, n_tensors); }
-
-extern "C" int niw_adam_step_tensors(const niw_adam_tensor* tensors, int64_t n_tensors, const niw_adam_hyper* hyper, int n_groups, double beta1, double beta2,
-                                     double eps, const float* hyper_dev, const float* decay_dev, const niw_adam_clip* clip, niw_stream_t stream) {
-    int rc = check_adam("niw_adam_step_tensors", tensors, n_tensors, n_groups);
+extern "C" int niw_adam_step_tensors(const niw_table* table, const niw_adam_hyper* hyper, double beta1, double beta2, double eps, const float* hyper_dev,
+                                     const float* decay_dev, const niw_adam_clip* clip, niw_stream_t stream) {
+    const int rc = check_table("niw_adam_step_tensors", table, table && table->form == kFormAdam);
     if (rc != NIW_OK) return rc;
     NIW_REQUIRE(hyper, "niw_adam_step_tensors: null pointer");
     NIW_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0, "niw_adam_step_tensors: beta1=%g beta2=%g eps=%g", beta1, beta2, eps);
-    AdamTable table{};
-    for (int k = 0; k < n_groups; ++k) {
+    AdamArgs a{};
+    for (int k = 0; k < table->groups; ++k) {
         const niw_adam_hyper& h = hyper[k];
         NIW_REQUIRE(h.step >= 1 || hyper_dev, "niw_adam_step_tensors: group %d step=%d", k, h.step);
         NIW_REQUIRE(isfinite(h.lr) && isfinite(h.weight_decay) && h.weight_decay >= 0.0, "niw_adam_step_tensors: group %d lr=%g weight_decay=%g", k, h.lr, h.weight_decay);
@@ -504,36 +672,27 @@ extern "C" int niw_adam_step_tensors(const niw_adam_tensor* tensors, int64_t n_t
         const int step = h.step < 1 ? 1 : h.step;
         // the scalars are formed in double and rounded to fp32 once, as in niw_adam_step
         const double bc1 = 1.0 - pow(beta1, (double)step), bc2 = 1.0 - pow(beta2, (double)step);
-        table.step_size[k] = (float)(h.lr / bc1);
-        table.bc2_sqrt[k] = (float)sqrt(bc2);
-        table.decay[k] = (float)(h.lr * h.weight_decay);
+        a.step_size[k] = (float)(h.lr / bc1);
+        a.bc2_sqrt[k] = (float)sqrt(bc2);
+        a.decay[k] = (float)(h.lr * h.weight_decay);
     }
-    table.w1 = (float)(1.0 - beta1); table.b2 = (float)beta2; table.w2 = (float)(1.0 - beta2); table.eps = (float)eps;
+    a.w1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.w2 = (float)(1.0 - beta2); a.eps = (float)eps;
+    a.hyper_dev = hyper_dev; a.decay_dev = decay_dev;
     hipStream_t st = (hipStream_t)stream;
-    const double* total = nullptr;
+    const auto list = list_of<AdamSlot>(*table);
+    const int64_t grid = grid_of(list, kAdamPart);
+    Clip c{};
     if (clip) {
         NIW_REQUIRE(clip->kind == NIW_NORM_2 || clip->kind == NIW_NORM_MAX, "niw_adam_step_tensors: unknown kind %d", clip->kind);
         NIW_REQUIRE(clip->max_norm >= 0.0, "niw_adam_step_tensors: max_norm=%g", clip->max_norm);
         NIW_REQUIRE(clip->total || clip->workspace, "niw_adam_step_tensors: null pointer");
-        total = clip->total;
-        if (!total) {
-            rc = total_of("niw_adam_step_tensors", tensors, n_tensors, fill_adam_grad, clip->kind, clip->workspace + 1, clip->workspace, nullptr, st);
-            if (rc != NIW_OK) return rc;
-            total = clip->workspace;
-        }
+        c.norm_out = clip->norm; c.max_norm = clip->max_norm; c.skip_nonfinite = clip->skip_nonfinite;
+        prepare_clip(c, list, *table, grid, clip->kind, clip->total, clip->workspace, st);
     }
-    const int kind = clip ? clip->kind : 0, skip = clip ? clip->skip_nonfinite : 0;
-    const double max_norm = clip ? clip->max_norm : 0.0;
-    float* const norm_out = clip ? clip->norm : nullptr;
-    bool launched = false;
-    rc = for_tables(tensors, n_tensors, table, fill_adam, [&](const AdamTable& t, long long) -> int {
-        adam_tensors_kernel<<<t.chunks, kThreads, 0, st>>>(t, hyper_dev, decay_dev, total, kind, skip, max_norm, launched ? nullptr : norm_out);
-        launched = true;
-        NIW_LAUNCH_CHECK("niw_adam_step_tensors");
-        return NIW_OK;
-    });
-    if (rc != NIW_OK || launched || !norm_out) return rc;
-    adam_tensors_kernel<<<1, kThreads, 0, st>>>(table, hyper_dev, decay_dev, total, kind, skip, max_norm, norm_out);      // (an empty list: the norm alone)
+    const bool nt = table->moved > kCache;
+    auto* const kernel = !clip || clip->kind == NIW_NORM_2 ? (nt ? adam_tensors_kernel<NIW_NORM_2, true> : adam_tensors_kernel<NIW_NORM_2, false>)
+                                                           : (nt ? adam_tensors_kernel<NIW_NORM_MAX, true> : adam_tensors_kernel<NIW_NORM_MAX, false>);
+    kernel<<<(unsigned)grid, kThreads, 0, st>>>(list, a, c);
     NIW_LAUNCH_CHECK("niw_adam_step_tensors");
     return NIW_OK;
 }

@@ -278,6 +278,7 @@ def adam_step_multi(groups, beta1=0.9, beta2=0.999, eps=1e-8, hyper_dev=None):
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}         # enum niw_dtype (include/niw.h)
 NORMS = {2.0: 0, math.inf: 1}                                             # enum niw_norm_kind
+NORM_WORKSPACE_DOUBLES = 1025
 
 
 def _norm_kind(norm_type):
@@ -324,21 +325,55 @@ def _check_device(tensors, name):
     return device
 
 
-def _checked(name, *args):
-    lib = _lib.load()
-    if getattr(lib, name)(*args):
-        raise _lib.NiwError(lib.niw_last_error_string().decode())
+def _on(device):
+    """makes the list's GPU current for a launch (its stream and allocations are that GPU's)"""
+    if device is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
-class TensorTable:
+class _Table:
+    """Device image of a list of tensors (niw_table).  The image is stored on the stream that is current when the table is built; a table that
+    is kept (`kept`) waits for that once, so that any stream may use it afterwards."""
+
+    def _build(self, name, entries, last, tensors, kept):
+        lib = _lib.load()
+        self._keep = [(t, t.untyped_storage()) for t in tensors]
+        host = ctypes.create_string_buffer(max(lib.niw_table_bytes(len(entries)), 16))
+        self._c = _lib.Table()
+        if getattr(lib, name)(entries, len(entries), last, host, ctypes.byref(self._c)):
+            raise _lib.NiwError(lib.niw_last_error_string().decode())
+        self._stream, self._image = None, None
+        if self._c.bytes:
+            if kept and torch.cuda.is_current_stream_capturing():
+                raise _lib.NiwError(f"{type(self).__name__}: build the table before the capture begins")
+            with _on(self.device):
+                self._image = torch.empty(self._c.bytes, device=self.device, dtype=torch.uint8)
+                self._c.image = self._image.data_ptr()
+                stream = torch.cuda.current_stream()
+                _lib.call("niw_table_store", host, self._c.bytes, _p(self._image), ctypes.c_void_p(stream.cuda_stream))
+                self._stream = stream.cuda_stream
+                if kept:
+                    stream.synchronize()
+
+    def _use(self):
+        """the current stream of the list's GPU, which the image is kept alive for"""
+        stream = torch.cuda.current_stream()
+        if self._image is not None and stream.cuda_stream != self._stream:
+            self._image.record_stream(stream)
+        return ctypes.c_void_p(stream.cuda_stream)
+
+
+class TensorTable(_Table):
     """What grad_norm / grad_total / clip_grads need to know of a list of tensors, gathered and checked once for tensors that stay where they
     are (a gradient bucket's views, gradients that are zeroed rather than dropped).  A plain list in its place is gathered at every call.
     tensors: float32 / bfloat16 / float16, mixed at will, each dense in any order, any length; None entries are left out.
     out: for clip_grads, one tensor per entry that receives the clipped values (same shape and order, any of the types); None: in place.
     The table speaks of the MEMORY the tensors had when it was built and keeps that memory alive; a tensor that is given other storage
-    afterwards (.grad re-created by a backward, .data re-assigned, .to()) is not followed: build a new table."""
+    afterwards (.grad re-created by a backward, .data re-assigned, .to()) is not followed: build a new table.  Building one waits for the GPU
+    once; any stream, thread or captured graph may use it then, several at a time (a graph does not keep it alive: the caller does)."""
 
-    def __init__(self, tensors, out=None):
+    def __init__(self, tensors, out=None, _kept=True):
         tensors = list(tensors)
         out = [None] * len(tensors) if out is None else list(out)
         if len(out) != len(tensors):
@@ -351,20 +386,21 @@ class TensorTable:
             if o is not None:
                 _check_dense(o, f"output {i}")
                 _check_same_layout(t, o, f"output {i}")
-        self.device = _check_device([x for p in pairs for x in p if x is not None], "TensorTable")
-        self.in_place = not pairs or pairs[0][1] is None
+        every = [x for p in pairs for x in p if x is not None]
+        self.device = _check_device(every, "TensorTable")
         self.numel = sum(t.numel() for t, _ in pairs)
-        self._keep = [(x, x.untyped_storage()) for p in pairs for x in p if x is not None]
-        self._n = len(pairs)
-        self._c = (_lib.GradTensor * max(self._n, 1))()
-        for c, (t, o) in zip(self._c, pairs):
+        entries = (_lib.GradTensor * len(pairs))()
+        for c, (t, o) in zip(entries, pairs):
             o = t if o is None else o
             c.grad, c.out, c.n, c.dtype, c.out_dtype = t.data_ptr(), o.data_ptr(), t.numel(), DTYPES[t.dtype], DTYPES[o.dtype]
-        _checked("niw_grad_check", self._c, self._n, 0)
-        self._overlap = _lib.load().niw_grad_check(self._c, self._n, 1) and _lib.load().niw_last_error_string().decode()
-        if self._overlap and not self.in_place:
-            raise _lib.NiwError(self._overlap)
-        self._doubles = _lib.load().niw_grad_workspace_doubles(self._c, self._n)
+        self._unclippable = None
+        try:
+            self._build("niw_grad_table", entries, 1, every, _kept)
+        except _lib.NiwError as e:
+            if pairs[0][1] is not None or "overlap" not in str(e):
+                raise
+            self._unclippable = str(e)               # tensors that share memory have a norm, but cannot be clipped in place
+            self._build("niw_grad_table", entries, 0, every, _kept)
 
 
 def _table(grads, out=None):
@@ -374,14 +410,11 @@ def _table(grads, out=None):
         return grads
     if isinstance(grads, torch.Tensor):
         grads, out = [grads], None if out is None else [out]
-    return TensorTable(grads, out)
+    return TensorTable(grads, out, _kept=False)
 
 
-def _on(device):
-    """makes the list's GPU current for a launch (its stream and allocations are that GPU's)"""
-    if device is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _norm_workspace(device):
+    return torch.empty(NORM_WORKSPACE_DOUBLES, device=device, dtype=torch.float64)
 
 
 def grad_total(grads, norm_type=2.0):
@@ -390,9 +423,9 @@ def grad_total(grads, norm_type=2.0):
     table, kind = _table(grads), _norm_kind(norm_type)
     with _on(table.device):
         total = torch.empty(1, device=table.device or "cuda", dtype=torch.float64)
-        ws = torch.empty(table._doubles, device=total.device, dtype=torch.float64)
+        ws = _norm_workspace(total.device)
         with timed("grad_norm", table.numel):
-            _lib.call("niw_grad_norm", table._c, table._n, kind, _p(ws), _p(total), None, _stream())
+            _lib.call("niw_grad_norm", ctypes.byref(table._c), kind, _p(ws), _p(total), None, table._use())
     return total
 
 
@@ -402,9 +435,9 @@ def grad_norm(grads, norm_type=2.0):
     table, kind = _table(grads), _norm_kind(norm_type)
     with _on(table.device):
         norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
-        ws = torch.empty(table._doubles, device=norm.device, dtype=torch.float64)
+        ws = _norm_workspace(norm.device)
         with timed("grad_norm", table.numel):
-            _lib.call("niw_grad_norm", table._c, table._n, kind, _p(ws), None, _p(norm), _stream())
+            _lib.call("niw_grad_norm", ctypes.byref(table._c), kind, _p(ws), None, _p(norm), table._use())
     return norm
 
 
@@ -431,18 +464,18 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None, total=None):
     the host.  total: the grad_total of all ranks where this rank holds a share; None: the norm of `grads` itself.
     In place nothing is written when nothing has to be clipped.  An infinite norm makes finite gradients 0, a NaN makes all of them NaN."""
     table, kind, max_norm = _table(grads, out), _norm_kind(norm_type), _max_norm(max_norm)
-    if table._overlap:
-        raise _lib.NiwError(table._overlap)
+    if table._unclippable:
+        raise _lib.NiwError(table._unclippable)
     total = _total(total, table.device)
     with _on(table.device):
         norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
-        ws = torch.empty(table._doubles, device=norm.device, dtype=torch.float64) if total is None else None
+        ws = _norm_workspace(norm.device) if total is None else None
         with timed("clip_grads", table.numel):
-            _lib.call("niw_grad_clip", table._c, table._n, kind, max_norm, _p(total), _p(ws), _p(norm), _stream())
+            _lib.call("niw_grad_clip", ctypes.byref(table._c), kind, max_norm, _p(total), _p(ws), _p(norm), table._use())
     return norm
 
 
-class AdamTable:
+class AdamTable(_Table):
     """What adam_step_tensors needs to know of its tensors, gathered and checked once (see TensorTable for what it keeps and does not follow).
     groups: up to 8 dicts of lists of equal length
         params      float32, or bfloat16 / float16 with `master`
@@ -451,7 +484,7 @@ class AdamTable:
         master      float32 copies that the update runs on (half-precision parameters receive the rounded result), None for float32
     The tensors of one entry have the same shape and the same order in memory."""
 
-    def __init__(self, groups):
+    def __init__(self, groups, _kept=True):
         groups = [dict(g) for g in groups]
         if not 1 <= len(groups) <= 8:
             raise _lib.NiwError(f"AdamTable: 1..8 groups (got {len(groups)})")
@@ -486,15 +519,12 @@ class AdamTable:
         self.device = _check_device(tensors, "AdamTable")
         self.n_groups = len(groups)
         self.numel = sum(row["params"].numel() for _, row in rows)
-        self._keep = [(t, t.untyped_storage()) for t in tensors]
-        self._n = len(rows)
-        self._c = (_lib.AdamTensor * max(self._n, 1))()
-        for c, (k, row) in zip(self._c, rows):
+        entries = (_lib.AdamTensor * len(rows))()
+        for c, (k, row) in zip(entries, rows):
             c.param, c.grad, c.exp_avg, c.exp_avg_sq = (row[key].data_ptr() for key in ("params", "grads", "exp_avg", "exp_avg_sq"))
             c.master = None if row["master"] is None else row["master"].data_ptr()
             c.n, c.param_dtype, c.grad_dtype, c.group = row["params"].numel(), DTYPES[row["params"].dtype], DTYPES[row["grads"].dtype], k
-        _checked("niw_adam_check", self._c, self._n, self.n_groups)
-        self._doubles = _lib.load().niw_adam_workspace_doubles(self._c, self._n)
+        self._build("niw_adam_table", entries, self.n_groups, tensors, _kept)
 
 
 def _per_group(value, n, name, kind):
@@ -513,7 +543,7 @@ def adam_step_tensors(tensors, lr, step, weight_decay=0.0, beta1=0.9, beta2=0.99
     skip_nonfinite (with max_norm): a norm that is not finite leaves everything as it was -- decided on the GPU, the host's step counts on.
     hyper_dev [n_groups, 2] = adam_hyper(lr, step) and decay_dev [n_groups] = lr * weight_decay (float32 device tensors): read by the kernel at
     run time instead of lr / step / weight_decay (graph replays)."""
-    table = tensors if isinstance(tensors, AdamTable) else AdamTable(tensors)
+    table = tensors if isinstance(tensors, AdamTable) else AdamTable(tensors, _kept=False)
     n = table.n_groups
     lr, step, decay = _per_group(lr, n, "lr", float), _per_group(step, n, "step", int), _per_group(weight_decay, n, "weight_decay", float)
     for t, shape, name in ((hyper_dev, 2 * n, "hyper_dev"), (decay_dev, n, "decay_dev")):
@@ -524,17 +554,18 @@ def adam_step_tensors(tensors, lr, step, weight_decay=0.0, beta1=0.9, beta2=0.99
         if skip_nonfinite or total is not None:
             raise _lib.NiwError("adam_step_tensors: skip_nonfinite and total go with max_norm (math.inf clips nothing)")
         with _on(table.device), timed("adam", table.numel):
-            _lib.call("niw_adam_step_tensors", table._c, table._n, hyper, n, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev), None, _stream())
+            _lib.call("niw_adam_step_tensors", ctypes.byref(table._c), hyper, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev), None,
+                      table._use())
         return None
     total, kind, max_norm = _total(total, table.device), _norm_kind(norm_type), _max_norm(max_norm)
     with _on(table.device):
         norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
-        ws = torch.empty(table._doubles, device=norm.device, dtype=torch.float64) if total is None else None
+        ws = _norm_workspace(norm.device) if total is None else None
         clip = _lib.AdamClip(max_norm=max_norm, kind=kind, skip_nonfinite=1 if skip_nonfinite else 0, total=None if total is None else total.data_ptr(),
                              workspace=None if ws is None else ws.data_ptr(), norm=norm.data_ptr())
         with timed("adam", table.numel):
-            _lib.call("niw_adam_step_tensors", table._c, table._n, hyper, n, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev),
-                      ctypes.byref(clip), _stream())
+            _lib.call("niw_adam_step_tensors", ctypes.byref(table._c), hyper, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev),
+                      ctypes.byref(clip), table._use())
     return norm
 
 

@@ -470,6 +470,53 @@ def test_captured_and_replayed():
             assert all(torch.equal(x, y) for x, y in zip(s[k], e[k])), (step, k)
 
 
+def test_a_table_is_built_in_front_of_a_capture_a_list_may_be_gathered_inside():
+    g = [rand(n, BF16, seed=n) for n in (70001, 3, 500)]
+    want = exact_norm(g)
+    ops.grad_norm(g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(_lib.NiwError, match="before the capture"):
+            ops.TensorTable(g)
+        norm = ops.grad_norm(g)                                              # its image is stored by the graph itself
+    for scale in (1.0, 2.0, 1.0):
+        for x, y in zip(g, [rand(n, BF16, seed=n) for n in (70001, 3, 500)]):
+            x.copy_(y * scale)
+        graph.replay()
+        junk = torch.full((1 << 20,), float("nan"), device=DEV)
+        torch.cuda.synchronize()
+        assert abs(float(norm) - scale * want) <= H * scale * want * 1.001
+        del junk
+
+
+def test_a_table_serves_streams_other_than_the_one_it_was_built_on():
+    g = [rand(n, F32, seed=n) for n in (300001, 5)]
+    want = exact_norm(g)
+    torch.cuda.synchronize()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        table = ops.TensorTable(g)
+    with torch.cuda.stream(other):
+        norm = ops.grad_norm(table)
+        del table                                                            # its memory is not handed out again before `other` has read it
+    with torch.cuda.stream(side):
+        junk = [torch.zeros(64, device=DEV, dtype=torch.uint8) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert abs(float(norm) - want) <= H * want * 1.001 and len(junk) == 8
+
+
+@pytest.mark.parametrize("count", [1, 2, 63, 64, 65, 127, 128, 129, 4095, 4096, 4097, 9000])
+def test_lists_of_many_tensors(count):
+    """every tensor of the list is found: each has a value of its own"""
+    flat = torch.arange(1, count + 1, device=DEV, dtype=F32)
+    g = [flat[i:i + 1] for i in range(count)]
+    want = math.sqrt(sum((i + 1) ** 2 for i in range(count)))
+    norm = ops.clip_grads(g, want / 2)
+    assert abs(float(norm) - want) <= H * want * 1.001
+    check_clipped(flat, torch.arange(1, count + 1, device=DEV, dtype=F32), coefficient(want, want / 2))
+
+
 def test_random_lists():
     """lists of random lengths, types and places in one buffer, against 64 bits"""
     r = random.Random(3)

@@ -20,6 +20,13 @@ def grads(*rows):
     return a
 
 
+def grad_table(rows, for_clip):
+    """-> (return code, table); the image goes nowhere near a GPU"""
+    lib = _lib.load()
+    image, t = ctypes.create_string_buffer(max(lib.niw_table_bytes(len(rows)), 16)), _lib.Table()
+    return lib.niw_grad_table(grads(*rows), len(rows), for_clip, image, ctypes.byref(t)), t
+
+
 @pytest.mark.parametrize("row,what", [
     ((None, None, 4, 0, 0), "null pointer"),
     ((1024, 1024, -1, 0, 0), "n=-1"),
@@ -28,11 +35,9 @@ def grads(*rows):
     ((1026, 1026, 4, 0, 0), "aligned"),
     ((1025, 1025, 4, 1, 1), "aligned"),
 ])
-def test_c_norm_and_clip_refuse_a_bad_descriptor(row, what):
-    lib = _lib.load()
-    a = grads(row)
-    for rc in (lib.niw_grad_check(a, 1, 0), lib.niw_grad_norm(a, 1, 0, 4096, 4096, None, None), lib.niw_grad_clip(a, 1, 0, 1.0, None, 4096, None, None)):
-        assert rc == -1 and what in err()
+def test_c_grad_table_refuses_a_bad_descriptor(row, what):
+    for for_clip in (0, 1):
+        assert grad_table([row], for_clip)[0] == -1 and what in err()
 
 
 @pytest.mark.parametrize("rows,what", [
@@ -41,10 +46,9 @@ def test_c_norm_and_clip_refuse_a_bad_descriptor(row, what):
     ([(1024, 2050, 4, 0, 0)], "aligned"),
     ([(1024, 1024, 4, 1, 0)], "changes its type"),
 ])
-def test_c_clip_refuses_a_bad_output(rows, what):
-    lib = _lib.load()
-    assert lib.niw_grad_clip(grads(*rows), len(rows), 0, 1.0, None, 4096, None, None) == -1 and what in err()
-    assert lib.niw_grad_check(grads(*rows), len(rows), 1) == -1 and what in err()
+def test_c_grad_table_for_clipping_refuses_a_bad_output(rows, what):
+    assert grad_table(rows, 1)[0] == -1 and what in err()
+    assert grad_table(rows, 0)[0] == 0                                        # (the norm does not look at outputs)
 
 
 @pytest.mark.parametrize("rows,ok", [
@@ -60,24 +64,50 @@ def test_c_clip_refuses_a_bad_output(rows, what):
     ([(8192, 8192, 4, 0, 0), (1024, 1024, 4000, 0, 0)], False),              # a long one from before
 ])
 def test_c_overlap_check(rows, ok):
-    lib = _lib.load()
-    rc = lib.niw_grad_check(grads(*rows), len(rows), 1)
+    rc, t = grad_table(rows, 1)
     assert (rc == 0) == ok and (ok or "overlap" in err())
-    assert lib.niw_grad_check(grads(*rows), len(rows), 0) == 0               # the norm may read whatever it likes
+    assert grad_table(rows, 0)[0] == 0                                        # the norm may read whatever it likes
 
 
-def test_c_norm_and_clip_refuse_bad_arguments():
+def test_c_table_counts_what_it_holds():
+    rc, t = grad_table([(1024, 1024, 4, 0, 0), (None, None, 0, 0, 0), (1 << 20, 1 << 20, 100000, 1, 1)], 1)
+    assert rc == 0 and t.slots == 2 and t.image is None and t.bytes % 16 == 0 and t.chunks == 1 + -(-100000 // t.chunk)
+    assert t.bytes <= _lib.load().niw_table_bytes(3)
+    rc, t = grad_table([(1 << 40, 1 << 40, 1 << 33, 0, 0)], 1)
+    assert rc == 0 and t.chunks == (1 << 33) // t.chunk
+    assert grad_table([], 1)[1].slots == 0
+    assert grad_table([(1024, 2048, 1 << 44, 0, 0)] * 3, 0)[0] == -1 and "chunks" in err()
+
+
+def test_c_calls_refuse_bad_arguments():
     lib = _lib.load()
-    a = grads((1024, 1024, 4, 0, 0))
-    assert lib.niw_grad_norm(a, 1, 2, 4096, 4096, None, None) == -1 and "kind 2" in err()
-    assert lib.niw_grad_norm(a, 1, 0, None, 4096, None, None) == -1 and "null pointer" in err()
-    assert lib.niw_grad_norm(a, 1, 0, 4096, None, None, None) == -1 and "null pointer" in err()
-    assert lib.niw_grad_norm(a, -1, 0, 4096, 4096, None, None) == -1 and "-1 tensors" in err()
-    assert lib.niw_grad_norm(None, 1, 0, 4096, 4096, None, None) == -1 and "null pointer" in err()
+    t = grad_table([(1024, 1024, 4, 0, 0)], 1)[1]
+    t.image = 4096
+    norm_only = grad_table([(1024, 1024, 4, 0, 0)], 0)[1]
+    norm_only.image = 4096
+    R = ctypes.byref
+    assert lib.niw_grad_table(None, 1, 0, 4096, R(_lib.Table())) == -1 and "1 tensors" in err()
+    assert lib.niw_grad_table(None, -1, 0, 4096, R(_lib.Table())) == -1 and "-1 tensors" in err()
+    assert lib.niw_grad_table(grads((1024, 1024, 4, 0, 0)), 1, 0, None, R(_lib.Table())) == -1 and "null pointer" in err()
+    assert lib.niw_table_bytes(-1) == 0
+    assert lib.niw_table_store(None, 16, 4096, None) == -1 and "null" in err()
+    assert lib.niw_table_store(4096, 16, 4097, None) == -1 and "misaligned" in err()
+    assert lib.niw_table_store(4096, 15, 4096, None) == -1 and "15 bytes" in err()
+    assert lib.niw_grad_norm(None, 0, 4096, 4096, None, None) == -1 and "null pointer" in err()
+    assert lib.niw_grad_norm(R(t), 2, 4096, 4096, None, None) == -1 and "kind 2" in err()
+    assert lib.niw_grad_norm(R(t), 0, None, 4096, None, None) == -1 and "null pointer" in err()
+    assert lib.niw_grad_norm(R(t), 0, 4096, None, None, None) == -1 and "null pointer" in err()
     for bad in (-1.0, math.nan, -math.inf):
-        assert lib.niw_grad_clip(a, 1, 0, bad, None, 4096, None, None) == -1 and "max_norm" in err()
-    assert lib.niw_grad_clip(a, 1, 5, 1.0, None, 4096, None, None) == -1 and "kind 5" in err()
-    assert lib.niw_grad_clip(a, 1, 0, 1.0, None, None, None, None) == -1 and "null pointer" in err()
+        assert lib.niw_grad_clip(R(t), 0, bad, None, 4096, None, None) == -1 and "max_norm" in err()
+    assert lib.niw_grad_clip(R(t), 5, 1.0, None, 4096, None, None) == -1 and "kind 5" in err()
+    assert lib.niw_grad_clip(R(t), 0, 1.0, None, None, None, None) == -1 and "null pointer" in err()
+    assert lib.niw_grad_clip(R(norm_only), 0, 1.0, None, 4096, None, None) == -1 and "form 1" in err()
+    t.image = None
+    assert lib.niw_grad_norm(R(t), 0, 4096, 4096, None, None) == -1 and "not stored" in err()
+    t.image = 4100
+    assert lib.niw_grad_norm(R(t), 0, 4096, 4096, None, None) == -1 and "not stored" in err()
+    h = (_lib.AdamHyper * 1)(_lib.AdamHyper(lr=1e-3, step=1))
+    assert lib.niw_adam_step_tensors(R(norm_only), h, 0.9, 0.999, 1e-8, None, None, None, None) == -1 and "form 1" in err()
 
 
 def adam_row(**kw):
@@ -87,27 +117,31 @@ def adam_row(**kw):
     return (_lib.AdamTensor * 1)(r)
 
 
+def adam_table(n_groups=1, **kw):
+    lib = _lib.load()
+    image, t = ctypes.create_string_buffer(lib.niw_table_bytes(1)), _lib.Table()
+    return lib.niw_adam_table(adam_row(**kw), 1, n_groups, image, ctypes.byref(t)), t
+
+
 @pytest.mark.parametrize("change,what", [
     (dict(param=None), "null pointer"), (dict(grad=None), "null pointer"), (dict(exp_avg=None), "null pointer"), (dict(exp_avg_sq=None), "null pointer"),
     (dict(n=-4), "n=-4"), (dict(param_dtype=5, master=16384), "dtype 5"), (dict(grad_dtype=-1), "dtype 0 / -1"), (dict(group=1), "group 1 of 1"),
     (dict(group=-1), "group -1"), (dict(master=16384), "master copy"), (dict(param_dtype=1), "master copy"), (dict(exp_avg=4098), "aligned"),
-    (dict(param_dtype=1, master=16385), "aligned"),
+    (dict(param_dtype=1, master=16385), "aligned"), (dict(n_groups=0), "1..8 groups"), (dict(n_groups=9), "1..8 groups"),
+    (dict(exp_avg=1024), "overlap"), (dict(exp_avg_sq=4100), "overlap"), (dict(grad=1024), "overlap"), (dict(param_dtype=1, master=1028), "overlap"),
 ])
-def test_c_adam_refuses_a_bad_descriptor(change, what):
-    lib = _lib.load()
-    h = (_lib.AdamHyper * 1)(_lib.AdamHyper(lr=1e-3, step=1))
-    assert lib.niw_adam_check(adam_row(**change), 1, 1) == -1 and what in err()
-    assert lib.niw_adam_step_tensors(adam_row(**change), 1, h, 1, 0.9, 0.999, 1e-8, None, None, None, None) == -1 and what in err()
+def test_c_adam_table_refuses(change, what):
+    assert adam_table(**change)[0] == -1 and what in err()
 
 
-def test_c_adam_refuses_bad_arguments_and_overlaps():
+def test_c_adam_refuses_bad_arguments():
     lib = _lib.load()
-    row = adam_row()
-    step = lambda h, n=1, b1=0.9, b2=0.999, eps=1e-8, hd=None, dd=None, clip=None: lib.niw_adam_step_tensors(row, 1, h, n, b1, b2, eps, hd, dd, clip, None)
+    rc, t = adam_table()
+    t.image = 4096
+    assert rc == 0
+    step = lambda h, b1=0.9, b2=0.999, eps=1e-8, hd=None, dd=None, clip=None: lib.niw_adam_step_tensors(ctypes.byref(t), h, b1, b2, eps, hd, dd, clip, None)
     H = lambda **kw: (_lib.AdamHyper * 1)(_lib.AdamHyper(**{**dict(lr=1e-3, weight_decay=0.0, step=1), **kw}))
     assert step(None) == -1 and "null pointer" in err()
-    assert step(H(), n=0) == -1 and "1..8 groups" in err()
-    assert step(H(), n=9) == -1 and "1..8 groups" in err()
     assert step(H(step=0)) == -1 and "step=0" in err()
     assert step(H(lr=math.nan)) == -1 and "lr=" in err()
     assert step(H(weight_decay=-0.1)) == -1 and "weight_decay" in err()
@@ -118,16 +152,6 @@ def test_c_adam_refuses_bad_arguments_and_overlaps():
     assert step(H(), clip=clip(max_norm=-1.0)) == -1 and "max_norm" in err()
     assert step(H(), clip=clip(kind=9)) == -1 and "kind 9" in err()
     assert step(H(), clip=clip(workspace=None)) == -1 and "null pointer" in err()
-    for kw in (dict(exp_avg=1024), dict(exp_avg_sq=4100), dict(grad=1024), dict(param_dtype=1, master=1028)):
-        assert lib.niw_adam_check(adam_row(**kw), 1, 1) == -1 and "overlap" in err()
-
-
-def test_workspace_queries_are_host_arithmetic():
-    lib = _lib.load()
-    assert lib.niw_grad_workspace_doubles(None, 0) >= 1
-    small = lib.niw_grad_workspace_doubles(grads((1024, 1024, 4, 0, 0)), 1)
-    assert 1 <= small <= lib.niw_grad_workspace_doubles(grads((1024, 1024, 1 << 34, 0, 0)), 1)
-    assert lib.niw_adam_workspace_doubles(adam_row(n=1 << 33), 1) >= 1
 
 
 # ------------------------------------------------------------------------------------------ Python wrappers (CPU tensors: refused last)
