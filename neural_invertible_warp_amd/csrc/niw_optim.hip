@@ -274,9 +274,12 @@ __device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, int head, l
     for (; i < end; ++i) seen(0, load1<DT>(p, i));
 }
 
-// chunks in front of `cached` are read past the caches: what a clip reads again is the end of the list
+template <int KIND>
+__device__ __forceinline__ double norm_of(double total) { return KIND == NIW_NORM_2 ? sqrt(total) : total; }
+
+// total, norm: for a launch of one workgroup, whose sum is the total; null otherwise.  Chunks in front of `cached` are read past the caches: what a clip reads again is the end of the list
 template <int KIND, class Slot>
-__global__ __launch_bounds__(kThreads) void partial_kernel(List<Slot> list, int cached, double* __restrict__ partial) {
+__global__ __launch_bounds__(kThreads) void partial_kernel(List<Slot> list, int cached, double* __restrict__ partial, double* __restrict__ total, float* __restrict__ norm) {
     Seen<KIND> seen;
     for_chunks(list, [&](const Slot& s, int c, int head, long long begin, long long end) {
         with_dtype(s.types & 255, [&](auto dt) {
@@ -285,7 +288,10 @@ __global__ __launch_bounds__(kThreads) void partial_kernel(List<Slot> list, int 
         });
     });
     const double sum = block_total<KIND>(seen.total());
-    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    if (threadIdx.x) return;
+    partial[blockIdx.x] = sum;
+    if (total) total[0] = sum;
+    if (norm) norm[0] = (float)norm_of<KIND>(sum);
 }
 
 // the total of n partial sums, in every thread: the same order wherever it is formed
@@ -296,9 +302,6 @@ __device__ __forceinline__ double total_of(const double* __restrict__ partial, i
     for (int i = threadIdx.x; i < n; i += kThreads) x = join<KIND>(x, partial[i]);
     return block_total<KIND>(x);
 }
-template <int KIND>
-__device__ __forceinline__ double norm_of(double total) { return KIND == NIW_NORM_2 ? sqrt(total) : total; }
-
 template <int KIND>
 __global__ __launch_bounds__(kThreads) void finish_kernel(const double* __restrict__ partial, int n, double* __restrict__ total, float* __restrict__ norm) {
     const double x = n ? total_of<KIND>(partial, n) : 0.0;
@@ -547,14 +550,16 @@ int check_table(const char* what, const niw_table* t, bool form_fits) {
     return NIW_OK;
 }
 
-// the launch that leaves the partial sums of the list in `partial`; -> their number
+// The launch that leaves the partial sums of the list in `partial`; -> their number.  One partial sum is the total, and goes to `total` and
+// `norm` (both may be null) at once.
 template <class Slot>
-int launch_partials(const List<Slot>& list, const niw_table& t, int kind, double* partial, hipStream_t st) {
+int launch_partials(const List<Slot>& list, const niw_table& t, int kind, double* partial, double* total, float* norm, hipStream_t st) {
     const int grid = list.chunks < kNormBlocks ? list.chunks : kNormBlocks;
     if (grid == 0) return 0;
     const int cached = t.read <= kCache ? 0 : (int)((double)list.chunks * (1.0 - (double)kCache / (double)t.read));
-    if (kind == NIW_NORM_2) partial_kernel<NIW_NORM_2><<<grid, kThreads, 0, st>>>(list, cached, partial);
-    else partial_kernel<NIW_NORM_MAX><<<grid, kThreads, 0, st>>>(list, cached, partial);
+    if (grid > 1) total = nullptr, norm = nullptr;
+    if (kind == NIW_NORM_2) partial_kernel<NIW_NORM_2><<<grid, kThreads, 0, st>>>(list, cached, partial, total, norm);
+    else partial_kernel<NIW_NORM_MAX><<<grid, kThreads, 0, st>>>(list, cached, partial, total, norm);
     return grid;
 }
 void launch_finish(int kind, const double* partial, int n, double* total, float* norm, hipStream_t st) {
@@ -572,7 +577,7 @@ void prepare_clip(Clip& clip, const List<Slot>& list, const niw_table& t, int64_
     clip.partial = total;
     clip.n_partial = 1;
     if (total) return;
-    const int n = launch_partials(list, t, kind, workspace + 1, st);
+    const int n = launch_partials(list, t, kind, workspace + 1, nullptr, nullptr, st);
     if (n > 0 && grid <= kFoldGrid) { clip.partial = workspace + 1; clip.n_partial = n; return; }
     launch_finish(kind, workspace + 1, n, workspace, nullptr, st);
     clip.partial = workspace;
@@ -622,8 +627,8 @@ extern "C" int niw_grad_norm(const niw_table* table, int kind, double* workspace
     NIW_REQUIRE(kind == NIW_NORM_2 || kind == NIW_NORM_MAX, "niw_grad_norm: unknown kind %d", kind);
     NIW_REQUIRE(workspace && (total || norm), "niw_grad_norm: null pointer");
     hipStream_t st = (hipStream_t)stream;
-    const int n = launch_partials(list_of<GradSlot>(*table), *table, kind, workspace + 1, st);
-    launch_finish(kind, workspace + 1, n, total, norm, st);
+    const int n = launch_partials(list_of<GradSlot>(*table), *table, kind, workspace + 1, total, norm, st);
+    if (n != 1) launch_finish(kind, workspace + 1, n, total, norm, st);
     NIW_LAUNCH_CHECK("niw_grad_norm");
     return NIW_OK;
 }

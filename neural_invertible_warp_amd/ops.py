@@ -357,11 +357,12 @@ class _Table:
                     stream.synchronize()
 
     def _use(self):
-        """the current stream of the list's GPU, which the image is kept alive for"""
-        stream = torch.cuda.current_stream()
-        if self._image is not None and stream.cuda_stream != self._stream:
-            self._image.record_stream(stream)
-        return ctypes.c_void_p(stream.cuda_stream)
+        """the current stream of the list's GPU (its handle alone: a torch.cuda.Stream object costs 2.5 us of a 14 us call), which the image is
+        kept alive for"""
+        handle = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+        if handle != self._stream and self._image is not None:
+            self._image.record_stream(torch.cuda.current_stream())
+        return handle
 
 
 class TensorTable(_Table):
