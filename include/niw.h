@@ -408,11 +408,14 @@ typedef struct niw_table {      /* HOST; everything but `image` is filled by niw
     int64_t read, moved;
 } niw_table;
 
+/* NIW_TABLE_CLIP: a table for niw_grad_clip too (without: for niw_grad_norm alone).  NIW_TABLE_KEPT: a table for many calls, whose image may
+ * cost more to store (up to 140 KB for a small list, of which every piece then has a slot of its own). */
+enum niw_table_flags { NIW_TABLE_CLIP = 1, NIW_TABLE_KEPT = 2 };
 /* bytes that hold the image of any list of n tensors */
 int64_t niw_table_bytes(int64_t n_tensors);
-/* image [niw_table_bytes(n_tensors)] HOST, overwritten; table: HOST, filled (image = NULL).  for_clip = 0: a table for niw_grad_norm; != 0: also for
- * niw_grad_clip, whose outputs must overlap neither each other nor a gradient (their own, in place, excepted).  Host arithmetic only. */
-int niw_grad_table(const niw_grad_tensor* tensors, int64_t n_tensors, int for_clip, void* image, niw_table* table);
+/* image [niw_table_bytes(n_tensors)] HOST, overwritten; table: HOST, filled (image = NULL).  With NIW_TABLE_CLIP the outputs must overlap neither
+ * each other nor a gradient (their own, in place, excepted).  Host arithmetic only. */
+int niw_grad_table(const niw_grad_tensor* tensors, int64_t n_tensors, int flags, void* image, niw_table* table);
 /* dst (device, `bytes` of the table) = the HOST image, which travels inside kernel arguments: stream-ordered, nothing of the host's has to
  * outlive the call, capturable. */
 int niw_table_store(const void* image, int64_t bytes, void* dst, niw_stream_t stream);
@@ -458,8 +461,8 @@ typedef struct niw_adam_clip {      /* HOST */
     double* workspace;          /* NIW_NORM_WORKSPACE_DOUBLES doubles (may be NULL with `total`) */
     float* norm;                /* [1] receives the norm, or NULL */
 } niw_adam_clip;
-/* as niw_grad_table; what is written (param, exp_avg, exp_avg_sq, master) must overlap nothing else of the list */
-int niw_adam_table(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups, void* image, niw_table* table);
+/* as niw_grad_table (flags: NIW_TABLE_KEPT or 0); what is written (param, exp_avg, exp_avg_sq, master) must overlap nothing else of the list */
+int niw_adam_table(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups, int flags, void* image, niw_table* table);
 /* hyper: HOST, one entry per group of the table.  hyper_dev: DEVICE array [n_groups][2] as in niw_adam_step_multi or NULL; decay_dev: DEVICE array
  * [n_groups] of lr * weight_decay or NULL: both replace what is formed from `hyper` and are read at run time (HIP-graph replays).
  * clip: NULL = the gradients as they are. */

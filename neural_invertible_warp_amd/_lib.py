@@ -129,7 +129,7 @@ SIGNATURES = {
     "niw_table_store": (_i, [_vp, _i64, _vp, _vp]),
     "niw_grad_norm": (_i, [_vp, _i, _vp, _vp, _vp, _vp]),
     "niw_grad_clip": (_i, [_vp, _i, _d, _vp, _vp, _vp, _vp]),
-    "niw_adam_table": (_i, [_vp, _i64, _i, _vp, _vp]),
+    "niw_adam_table": (_i, [_vp, _i64, _i, _i, _vp, _vp]),
     "niw_adam_step_tensors": (_i, [_vp, _vp, _d, _d, _d, _vp, _vp, _vp, _vp]),
     "niw_train_step_prepare": (_i, []),
     "niw_train_step_workspace_floats": (_i64, [ctypes.POINTER(TrainDesc)]),

@@ -31,6 +31,8 @@ constexpr double kClipEps = 1e-6;
 // trainer's 1.2 M: clip 17 -> 15 us, of 1000 vectors alike with either).
 constexpr int kChunk = 16384, kSmallChunk = 4096;
 constexpr long long kSmallList = 1024ll * kChunk;
+constexpr int kMaxPieces = 2048;               // (of a kept small list: see build)
+constexpr int kRound = 2048;
 // The norm runs on at most kNormBlocks workgroups, four per compute unit, that walk the list with its whole width: 1 GB and up read at
 // 7.0 TB/s with 1024, 6.7 with 2048 or 4096, 6.8 with 512 (which costs half-precision lists a quarter: their conversions want more waves).
 constexpr int kNormBlocks = 1024;
@@ -48,7 +50,6 @@ constexpr int kFoldGrid = 4096;
 // Lists that move more than the 256 MB of memory-side cache hold go past the caches (non-temporal); a norm still leaves the last
 // kCache bytes of gradients in it, which the clip or update behind it reads first: it walks the list backwards.
 constexpr int64_t kCache = 192ll << 20;
-
 
 // ------------------------------------------------------------------------------------------------ the image of a list
 enum Form { kFormNorm = 1, kFormClip = 2, kFormAdam = 3 };
@@ -77,7 +78,8 @@ template <class Slot>
 struct List {
     const Slot* slots;
     int count, chunks, chunk;
-    __device__ const int* first() const { return reinterpret_cast<const int*>(slots + count); }
+    // the slot of chunk c: its own number in a list whose tensors have a chunk each
+    __device__ __forceinline__ int slot_of(int c) const;
 };
 
 // The tensor that chunk c belongs to: every lane looks at one of 64 evenly spaced tensors and the vote of the wave narrows the list to
@@ -93,6 +95,11 @@ __device__ __forceinline__ int find_slot(const int* first, int count, int c) {
         n = min(stride, n - k * stride);
     }
     return __builtin_amdgcn_readfirstlane(lo);
+}
+
+template <class Slot>
+__device__ __forceinline__ int List<Slot>::slot_of(int c) const {
+    return count == chunks ? c : find_slot(reinterpret_cast<const int*>(slots + count), count, c);
 }
 
 // A tensor's first chunk begins with its `head`: the elements in front of the first 128-byte boundary of the stream that matters most (the
@@ -123,7 +130,7 @@ __device__ __forceinline__ void for_chunks(const List<Slot>& list, F f) {
     Slot s{};
     for (int c = blockIdx.x; c < list.chunks; c += gridDim.x) {
         if (c < lo || c >= hi) {
-            s = list.slots[find_slot(list.first(), list.count, c)];
+            s = list.slots[list.slot_of(c)];
             lo = s.first;
             hi = lo + (int)chunks_of(s, list.chunk);
             head = head_of(s, false);
@@ -133,21 +140,45 @@ __device__ __forceinline__ void for_chunks(const List<Slot>& list, F f) {
         if (begin < s.n) f(s, c, begin == 0 ? head : 0, begin, end < s.n ? end : s.n);
     }
 }
-// parts of at most `part` elements that a chunk is cut into
+// The element of [begin, end) that this thread handles alone, or -1: the `head` ones in front of the aligned stretch (threads 0 ..), and
+// those behind the last whole vector of V (threads 128 ..).  One element per thread, so that they wait for memory once together.
+template <int V>
+__device__ __forceinline__ long long odd_element(int head, long long begin, long long end) {
+    static_assert(kLine / 2 <= kThreads / 2 && V <= kThreads / 2, "a thread per element");
+    const int tid = threadIdx.x, tail = (int)((end - begin - head) % V);
+    if (tid < head) return begin + tid;
+    return tid >= kThreads / 2 && tid < kThreads / 2 + tail ? end - tail + (tid - kThreads / 2) : -1;
+}
+// Parts of `part` elements that a chunk is cut into; in small lists no more than one round of workgroups, eight per compute unit (Adam of
+// 600 vectors 16.7 -> 14.3 us).
 template <class Slot>
 __host__ __device__ inline int parts_of(const List<Slot>& list, int part) {
-    return list.chunk > part ? list.chunk / part : 1;
+    int n = list.chunk > part ? list.chunk / part : 1;
+    while (list.chunk == kSmallChunk && n > 1 && list.chunks * n > kRound) n /= 2;
+    return n;
 }
-// f(slot, head, begin, end) for the part of this workgroup (one workgroup per part), from the list's end backwards
-template <int PART, class Slot, class F>
-__device__ __forceinline__ void for_part(const List<Slot>& list, F f) {
+// the part of this workgroup (one workgroup per part), from the list's end backwards; any = false: nothing is left for it
+template <class Slot>
+struct Part {
+    Slot s;
+    long long begin, end;
+    int head;
+    bool any;
+};
+template <int PART, class Slot>
+__device__ __forceinline__ Part<Slot> part_of(const List<Slot>& list) {
     const int split = parts_of(list, PART), b = (int)blockIdx.x / split, part = split - 1 - (int)blockIdx.x % split;
     const int c = list.chunks - 1 - b;
-    if (c < 0) return;
-    const Slot s = list.slots[find_slot(list.first(), list.count, c)];
-    const int head = head_of(s, true), step = list.chunk / split;
-    const long long at = (long long)(c - s.first) * list.chunk + part * step, begin = at == 0 ? 0 : head + at, end = head + at + step;
-    if (begin < s.n) f(s, begin == 0 ? head : 0, begin, end < s.n ? end : s.n);
+    Part<Slot> p{};
+    if (c < 0) return p;
+    p.s = list.slots[list.slot_of(c)];
+    const int head = head_of(p.s, true), step = list.chunk / split;
+    const long long at = (long long)(c - p.s.first) * list.chunk + part * step;
+    p.head = at == 0 ? head : 0;
+    p.begin = at == 0 ? 0 : head + at;
+    p.end = head + at + step < p.s.n ? head + at + step : p.s.n;
+    p.any = p.begin < p.s.n;
+    return p;
 }
 
 // ------------------------------------------------------------------------------------------------ elements
@@ -261,7 +292,8 @@ __device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, int head, l
             else { seen(2 * k, widen<DT>((unsigned short)bits)); seen(2 * k + 1, widen<DT>((unsigned short)(bits >> 16))); }
         }
     };
-    if (tid < head) seen(0, load1<DT>(p, tid));
+    const long long odd = odd_element<V>(head, begin, end);
+    const float alone = odd >= 0 ? load1<DT>(p, odd) : 0.f;
     long long i = begin + head;
     for (; i + (long long)kThreads * V * U <= end; i += (long long)kThreads * V * U) {
         u32x4 w[U];
@@ -271,7 +303,7 @@ __device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, int head, l
         for (int u = 0; u < U; ++u) take(w[u]);
     }
     for (i += tid * V; i + V <= end; i += kThreads * V) take(words(i));
-    for (; i < end; ++i) seen(0, load1<DT>(p, i));
+    seen(0, alone);
 }
 
 template <int KIND>
@@ -318,41 +350,43 @@ struct Clip {
     double max_norm;
     int n_partial, skip_nonfinite;
 };
-// -> the factor; `skip`: leave everything as it is
+struct Factor {
+    float c;
+    bool skip;                                // leave everything as it is
+};
 template <int KIND>
-__device__ __forceinline__ float clip_factor(const Clip& clip, bool& skip) {
-    skip = false;
-    if (!clip.partial) return 1.f;
+__device__ __forceinline__ Factor clip_factor(const Clip& clip) {
+    if (!clip.partial) return Factor{1.f, false};
     const double norm = norm_of<KIND>(total_of<KIND>(clip.partial, clip.n_partial));
     if (clip.norm_out && blockIdx.x == 0 && threadIdx.x == 0) clip.norm_out[0] = (float)norm;
-    skip = clip.skip_nonfinite && !isfinite(norm);
-    if (isinf(clip.max_norm)) return 1.f;
+    Factor f{1.f, clip.skip_nonfinite && !isfinite(norm)};
+    if (isinf(clip.max_norm)) return f;
     const double c = clip.max_norm / (norm + kClipEps);
-    return c < 1.0 || c != c ? (float)c : 1.f;
+    if (c < 1.0 || c != c) f.c = (float)c;
+    return f;
 }
 
 template <int KIND, bool NT, int PART>
 __global__ __launch_bounds__(kThreads) void clip_kernel(List<GradSlot> list, Clip clip) {
-    bool skip;
-    const float c = clip_factor<KIND>(clip, skip);
-    for_part<PART>(list, [&](const GradSlot& s, int head, long long begin, long long end) {
-        if (c == 1.f && s.o == s.g) return;
-        with_dtype(s.types & 255, [&](auto gt) {
-            with_dtype(s.types >> 8, [&](auto ot) {
-                constexpr int G = decltype(gt)::value, O = decltype(ot)::value, U = PART / (kThreads * 4);
-                const int tid = threadIdx.x;
-                if (tid < head) store1<O>(s.o, tid, c * load1<G>(s.g, tid));
-                long long i = begin + head;
-                for (; i + kThreads * 4 * U <= end; i += kThreads * 4 * U) {
-                    f32x4 x[U];
+    const float c = clip_factor<KIND>(clip).c;
+    const auto part = part_of<PART>(list);
+    const GradSlot& s = part.s;
+    if (!part.any || (c == 1.f && s.o == s.g)) return;
+    with_dtype(s.types & 255, [&](auto gt) {
+        with_dtype(s.types >> 8, [&](auto ot) {
+            constexpr int G = decltype(gt)::value, O = decltype(ot)::value, U = PART / (kThreads * 4);
+            const int tid = threadIdx.x;
+            const long long odd = odd_element<4>(part.head, part.begin, part.end);
+            if (odd >= 0) store1<O>(s.o, odd, c * load1<G>(s.g, odd));
+            long long i = part.begin + part.head;
+            for (; i + kThreads * 4 * U <= part.end; i += kThreads * 4 * U) {
+                f32x4 x[U];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) x[u] = load4<NT, G>(s.g, i + (u * kThreads + tid) * 4);
+                for (int u = 0; u < U; ++u) x[u] = load4<NT, G>(s.g, i + (u * kThreads + tid) * 4);
 #pragma unroll
-                    for (int u = 0; u < U; ++u) store4<NT, O>(s.o, i + (u * kThreads + tid) * 4, c * x[u]);
-                }
-                for (i += tid * 4; i + 4 <= end; i += kThreads * 4) store4<NT, O>(s.o, i, c * load4<NT, G>(s.g, i));
-                for (; i < end; ++i) store1<O>(s.o, i, c * load1<G>(s.g, i));
-            });
+                for (int u = 0; u < U; ++u) store4<NT, O>(s.o, i + (u * kThreads + tid) * 4, c * x[u]);
+            }
+            for (i += tid * 4; i + 4 <= part.end; i += kThreads * 4) store4<NT, O>(s.o, i, c * load4<NT, G>(s.g, i));
         });
     });
 }
@@ -366,46 +400,47 @@ struct AdamArgs {
 
 template <int KIND, bool NT>
 __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> list, AdamArgs a, Clip clip) {
-    bool skip;
-    const float c = clip_factor<KIND>(clip, skip);
-    if (skip) return;
-    for_part<kAdamPart>(list, [&](const AdamSlot& s, int head, long long begin, long long end) {
-        const int k = __builtin_amdgcn_readfirstlane(s.types >> 16);
-        const float step_size = a.hyper_dev ? a.hyper_dev[2 * k] : a.step_size[k], bc2_sqrt = a.hyper_dev ? a.hyper_dev[2 * k + 1] : a.bc2_sqrt[k];
-        const float decay = a.decay_dev ? a.decay_dev[k] : a.decay[k];
-        float* const w = s.w ? s.w : static_cast<float*>(s.p);
-        auto update = [&](float& p, float g, float& m, float& v) {
-            p = fmaf(-decay, p, p);
-            niw::adam_update(p, niw::mul_rn(c, g), m, v, a.w1, a.b2, a.w2, a.eps, step_size, bc2_sqrt);
-        };
-        with_dtype(s.types & 255, [&](auto gt) {
-            with_dtype((s.types >> 8) & 255, [&](auto pt) {
-                constexpr int G = decltype(gt)::value, P = decltype(pt)::value;
-                auto one = [&](long long i) {
-                    float p = w[i], m = s.m[i], v = s.v[i];
-                    update(p, load1<G>(s.g, i), m, v);
-                    w[i] = p; s.m[i] = m; s.v[i] = v;
-                    if constexpr (P != NIW_F32) store1<P>(s.p, i, p);
-                };
-                const int tid = threadIdx.x;
-                if (tid < head) one(tid);
-                long long i = begin + head + tid * 4;
-                for (; i + 4 <= end; i += kThreads * 4) {
-                    f32x4 p = load4<NT, NIW_F32>(w, i), m = load4<NT, NIW_F32>(s.m, i), v = load4<NT, NIW_F32>(s.v, i);
-                    const f32x4 g = load4<NT, G>(s.g, i);
+    const Factor factor = clip_factor<KIND>(clip);
+    const auto part = part_of<kAdamPart>(list);
+    if (!part.any || factor.skip) return;
+    const AdamSlot& s = part.s;
+    const int k = __builtin_amdgcn_readfirstlane(s.types >> 16), tid = threadIdx.x;
+    const float step_size = a.hyper_dev ? a.hyper_dev[2 * k] : a.step_size[k], bc2_sqrt = a.hyper_dev ? a.hyper_dev[2 * k + 1] : a.bc2_sqrt[k];
+    const float decay = a.decay_dev ? a.decay_dev[k] : a.decay[k];
+    float* const w = s.w ? s.w : static_cast<float*>(s.p);
+    with_dtype(s.types & 255, [&](auto gt) {
+        with_dtype((s.types >> 8) & 255, [&](auto pt) {
+            constexpr int G = decltype(gt)::value, P = decltype(pt)::value;
+            struct Four {
+                f32x4 p, m, v, g;
+            };
+            auto read = [&](long long i) {
+                return Four{load4<NT, NIW_F32>(w, i), load4<NT, NIW_F32>(s.m, i), load4<NT, NIW_F32>(s.v, i), load4<NT, G>(s.g, i)};
+            };
+            auto update = [&](float& p, float g, float& m, float& v) {
+                p = fmaf(-decay, p, p);
+                niw::adam_update(p, niw::mul_rn(factor.c, g), m, v, a.w1, a.b2, a.w2, a.eps, step_size, bc2_sqrt);
+            };
+            const long long odd = odd_element<4>(part.head, part.begin, part.end);
+            if (odd >= 0) {
+                float p = w[odd], m = s.m[odd], v = s.v[odd];
+                update(p, load1<G>(s.g, odd), m, v);
+                w[odd] = p; s.m[odd] = m; s.v[odd] = v;
+                if constexpr (P != NIW_F32) store1<P>(s.p, odd, p);
+            }
+            for (long long i = part.begin + part.head + tid * 4; i + 4 <= part.end; i += kThreads * 4) {
+                Four x = read(i);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float pj = p[j], mj = m[j], vj = v[j];
-                        update(pj, g[j], mj, vj);
-                        p[j] = pj; m[j] = mj; v[j] = vj;
-                    }
-                    store4<NT, NIW_F32>(w, i, p);
-                    store4<NT, NIW_F32>(s.m, i, m);
-                    store4<NT, NIW_F32>(s.v, i, v);
-                    if constexpr (P != NIW_F32) store4<NT, P>(s.p, i, p);
+                for (int j = 0; j < 4; ++j) {
+                    float pj = x.p[j], mj = x.m[j], vj = x.v[j];
+                    update(pj, x.g[j], mj, vj);
+                    x.p[j] = pj; x.m[j] = mj; x.v[j] = vj;
                 }
-                for (; i < end; ++i) one(i);
-            });
+                store4<NT, NIW_F32>(w, i, x.p);
+                store4<NT, NIW_F32>(s.m, i, x.m);
+                store4<NT, NIW_F32>(s.v, i, x.v);
+                if constexpr (P != NIW_F32) store4<NT, P>(s.p, i, x.p);
+            }
         });
     });
 }
@@ -510,32 +545,64 @@ void read_written(const niw_adam_tensor& t, int64_t& read, int64_t& moved) {
     read += t.n * size_of(t.grad_dtype); moved += t.n * (24 + size_of(t.grad_dtype) + (t.master ? 2 : 0));
 }
 
+// the elements [at, at + n) of a slot
+void advance(GradSlot& s, long long at, long long n) {
+    s.g = static_cast<const char*>(s.g) + at * size_of(s.types & 255);
+    s.o = static_cast<char*>(s.o) + at * size_of(s.types >> 8);
+    s.n = n;
+}
+void advance(AdamSlot& s, long long at, long long n) {
+    s.p = static_cast<char*>(s.p) + at * size_of((s.types >> 8) & 255);
+    s.g = static_cast<const char*>(s.g) + at * size_of(s.types & 255);
+    s.m += at; s.v += at;
+    if (s.w) s.w += at;
+    s.n = n;
+}
+
 template <class Slot, class Item>
-int build(const char* what, const Item* items, int64_t count, int form, int groups, void* image, niw_table* table) {
-    long long total = 0;
+int build(const char* what, const Item* items, int64_t count, int form, int groups, bool kept, void* image, niw_table* table) {
+    long long total = 0, pieces = 0;
     int slots = 0;
     *table = niw_table{};
     for (int64_t i = 0; i < count; ++i) {
         total += items[i].n; slots += items[i].n > 0;
+        pieces += items[i].n / (kSmallChunk - kLine) + 1;
         read_written(items[i], table->read, table->moved);
     }
-    table->form = form; table->slots = slots; table->groups = groups;
-    table->chunk = total < kSmallList ? kSmallChunk : kChunk;
-    table->bytes = padded((int64_t)slots * (sizeof(Slot) + sizeof(int)));
-    memset(image, 0, table->bytes);
-    Slot* s = static_cast<Slot*>(image);
-    int* first = reinterpret_cast<int*>(s + slots);
+    const int chunk = total < kSmallList ? kSmallChunk : kChunk;
+    // small lists that are kept: a slot per chunk, so that no workgroup has to search
+    const bool cut = kept && chunk == kSmallChunk && pieces <= kMaxPieces;
+    std::vector<Slot> list;
+    list.reserve(cut ? pieces : slots);
     long long chunks = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (items[i].n == 0) continue;
-        fill(*s, items[i]);
-        s->first = *first = (int)chunks;
-        chunks += chunks_of(*s, table->chunk);
-        ++s; ++first;
-        NIW_REQUIRE(chunks <= kMaxChunks, "%s: more than %lld chunks of %d elements", what, (long long)kMaxChunks, table->chunk);
+        Slot whole{};
+        fill(whole, items[i]);
+        for (long long at = 0, n; at < items[i].n; at += n) {
+            n = items[i].n - at;
+            if (cut) {
+                // (a first piece ends where the written stream begins a line)
+                const int head = at == 0 ? head_of(whole, form != kFormNorm) : 0;
+                n = std::min<long long>(n, head ? head + chunk - kLine : chunk);
+            }
+            Slot s = whole;
+            advance(s, at, n);
+            s.first = (int)chunks;
+            list.push_back(s);
+            chunks += chunks_of(s, chunk);
+            NIW_REQUIRE(chunks <= kMaxChunks, "%s: more than %lld chunks of %d elements", what, (long long)kMaxChunks, chunk);
+        }
     }
-    table->chunks = (int)chunks;
+    slots = (int)list.size();
+    table->form = form; table->slots = slots; table->chunks = (int)chunks; table->chunk = chunk; table->groups = groups;
     table->wide = table->moved >= 8 * total;
+    table->bytes = padded((int64_t)slots * (sizeof(Slot) + sizeof(int)));
+    if (!slots) return NIW_OK;
+    memset(image, 0, table->bytes);
+    memcpy(image, list.data(), slots * sizeof(Slot));
+    int* first = reinterpret_cast<int*>(static_cast<Slot*>(image) + slots);
+    for (int i = 0; i < slots; ++i) first[i] = list[i].first;
     return NIW_OK;
 }
 
@@ -585,24 +652,27 @@ void prepare_clip(Clip& clip, const List<Slot>& list, const niw_table& t, int64_
 
 }  // namespace
 
-extern "C" int64_t niw_table_bytes(int64_t n_tensors) { return n_tensors < 0 ? 0 : padded(n_tensors * (int64_t)(sizeof(AdamSlot) + sizeof(int))); }
+extern "C" int64_t niw_table_bytes(int64_t n_tensors) { return n_tensors < 0 ? 0 : padded((n_tensors + kMaxPieces) * (int64_t)(sizeof(AdamSlot) + sizeof(int))); }
 
-extern "C" int niw_grad_table(const niw_grad_tensor* tensors, int64_t n_tensors, int for_clip, void* image, niw_table* table) try {
+extern "C" int niw_grad_table(const niw_grad_tensor* tensors, int64_t n_tensors, int flags, void* image, niw_table* table) try {
     NIW_REQUIRE(n_tensors >= 0 && n_tensors <= kMaxTensors && (tensors || n_tensors == 0), "niw_grad_table: %lld tensors at %p", (long long)n_tensors, (const void*)tensors);
     NIW_REQUIRE(table && (image || n_tensors == 0), "niw_grad_table: null pointer");
-    const int rc = check_grads("niw_grad_table", tensors, n_tensors, for_clip != 0);
-    return rc != NIW_OK ? rc : build<GradSlot>("niw_grad_table", tensors, n_tensors, for_clip ? kFormClip : kFormNorm, 0, image, table);
+    NIW_REQUIRE((flags & ~(NIW_TABLE_CLIP | NIW_TABLE_KEPT)) == 0, "niw_grad_table: flags %d", flags);
+    const bool for_clip = (flags & NIW_TABLE_CLIP) != 0;
+    const int rc = check_grads("niw_grad_table", tensors, n_tensors, for_clip);
+    return rc != NIW_OK ? rc : build<GradSlot>("niw_grad_table", tensors, n_tensors, for_clip ? kFormClip : kFormNorm, 0, (flags & NIW_TABLE_KEPT) != 0, image, table);
 } catch (...) {
     niw_set_error("niw_grad_table: out of host memory");
     return NIW_ERR_INVALID_ARG;
 }
 
-extern "C" int niw_adam_table(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups, void* image, niw_table* table) try {
+extern "C" int niw_adam_table(const niw_adam_tensor* tensors, int64_t n_tensors, int n_groups, int flags, void* image, niw_table* table) try {
     NIW_REQUIRE(n_tensors >= 0 && n_tensors <= kMaxTensors && (tensors || n_tensors == 0), "niw_adam_table: %lld tensors at %p", (long long)n_tensors, (const void*)tensors);
     NIW_REQUIRE(table && (image || n_tensors == 0), "niw_adam_table: null pointer");
+    NIW_REQUIRE((flags & ~NIW_TABLE_KEPT) == 0, "niw_adam_table: flags %d", flags);
     NIW_REQUIRE(n_groups >= 1 && n_groups <= NIW_ADAM_MAX_GROUPS, "niw_adam_table: 1..%d groups (got %d)", NIW_ADAM_MAX_GROUPS, n_groups);
     const int rc = check_adam("niw_adam_table", tensors, n_tensors, n_groups);
-    return rc != NIW_OK ? rc : build<AdamSlot>("niw_adam_table", tensors, n_tensors, kFormAdam, n_groups, image, table);
+    return rc != NIW_OK ? rc : build<AdamSlot>("niw_adam_table", tensors, n_tensors, kFormAdam, n_groups, (flags & NIW_TABLE_KEPT) != 0, image, table);
 } catch (...) {
     niw_set_error("niw_adam_table: out of host memory");
     return NIW_ERR_INVALID_ARG;

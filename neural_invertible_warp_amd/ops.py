@@ -279,6 +279,7 @@ def adam_step_multi(groups, beta1=0.9, beta2=0.999, eps=1e-8, hyper_dev=None):
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}         # enum niw_dtype (include/niw.h)
 NORMS = {2.0: 0, math.inf: 1}                                             # enum niw_norm_kind
 NORM_WORKSPACE_DOUBLES = 1025
+TABLE_CLIP, TABLE_KEPT = 1, 2                                             # enum niw_table_flags
 
 
 def _norm_kind(norm_type):
@@ -336,12 +337,12 @@ class _Table:
     """Device image of a list of tensors (niw_table).  The image is stored on the stream that is current when the table is built; a table that
     is kept (`kept`) waits for that once, so that any stream may use it afterwards."""
 
-    def _build(self, name, entries, last, tensors, kept):
+    def _build(self, name, entries, how, tensors, kept):
         lib = _lib.load()
         self._keep = [(t, t.untyped_storage()) for t in tensors]
         host = ctypes.create_string_buffer(max(lib.niw_table_bytes(len(entries)), 16))
         self._c = _lib.Table()
-        if getattr(lib, name)(entries, len(entries), last, host, ctypes.byref(self._c)):
+        if getattr(lib, name)(entries, len(entries), *how, host, ctypes.byref(self._c)):
             raise _lib.NiwError(lib.niw_last_error_string().decode())
         self._stream, self._image = None, None
         if self._c.bytes:
@@ -396,12 +397,12 @@ class TensorTable(_Table):
             c.grad, c.out, c.n, c.dtype, c.out_dtype = t.data_ptr(), o.data_ptr(), t.numel(), DTYPES[t.dtype], DTYPES[o.dtype]
         self._unclippable = None
         try:
-            self._build("niw_grad_table", entries, 1, every, _kept)
+            self._build("niw_grad_table", entries, (TABLE_CLIP | (TABLE_KEPT if _kept else 0),), every, _kept)
         except _lib.NiwError as e:
             if pairs[0][1] is not None or "overlap" not in str(e):
                 raise
             self._unclippable = str(e)               # tensors that share memory have a norm, but cannot be clipped in place
-            self._build("niw_grad_table", entries, 0, every, _kept)
+            self._build("niw_grad_table", entries, (TABLE_KEPT if _kept else 0,), every, _kept)
 
 
 def _table(grads, out=None):
@@ -525,7 +526,7 @@ class AdamTable(_Table):
             c.param, c.grad, c.exp_avg, c.exp_avg_sq = (row[key].data_ptr() for key in ("params", "grads", "exp_avg", "exp_avg_sq"))
             c.master = None if row["master"] is None else row["master"].data_ptr()
             c.n, c.param_dtype, c.grad_dtype, c.group = row["params"].numel(), DTYPES[row["params"].dtype], DTYPES[row["grads"].dtype], k
-        self._build("niw_adam_table", entries, self.n_groups, tensors, _kept)
+        self._build("niw_adam_table", entries, (self.n_groups, TABLE_KEPT if _kept else 0), tensors, _kept)
 
 
 def _per_group(value, n, name, kind):

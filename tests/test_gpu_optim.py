@@ -54,16 +54,18 @@ def check_clipped(out, before, c):
 
 
 LENGTHS = [[1], [2, 1], [255], [256], [257], [1023, 1025], [16383], [16384], [16385], [65537], [0, 5, 0, 16384 * 3 + 1], [1000003], [7] * 250, [3, 70001] * 61,
-           [0]]
+           [0], [17_000_003], [9_000_001, 1, 8_388_608]]
 
 
 @pytest.mark.parametrize("kind", [2.0, math.inf])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lengths", LENGTHS, ids=lambda v: f"{len(v)}x{max(v)}")
-def test_norm(lengths, dtype, kind):
+@pytest.mark.parametrize("kept", [False, True])
+def test_norm(lengths, dtype, kind, kept):
     tensors = [rand(n, dtype, seed=i, offset=i % 3) for i, n in enumerate(lengths)]
-    check_norm(ops.grad_norm(tensors, norm_type=kind), tensors, kind)
-    total = ops.grad_total(tensors, norm_type=kind)
+    given = ops.TensorTable(tensors) if kept else tensors
+    check_norm(ops.grad_norm(given, norm_type=kind), tensors, kind)
+    total = ops.grad_total(given, norm_type=kind)
     assert total.dtype == torch.float64 and total.shape == (1,)
     want = exact_norm(tensors, kind) ** (2 if kind == 2.0 else 1)
     assert abs(float(total) - want) <= 1e-12 * want
@@ -131,13 +133,14 @@ OUTS = [(F32, None), (BF16, None), (F16, None), (F32, F32), (BF16, F32), (F16, F
 @pytest.mark.parametrize("kind", [2.0, math.inf])
 @pytest.mark.parametrize("dtype,out_dtype", OUTS, ids=str)
 @pytest.mark.parametrize("lengths", LENGTHS, ids=lambda v: f"{len(v)}x{max(v)}")
-def test_clip(lengths, dtype, out_dtype, kind):
+@pytest.mark.parametrize("kept", [False, True])
+def test_clip(lengths, dtype, out_dtype, kind, kept):
     before = [rand(n, dtype, seed=i, offset=i % 3) for i, n in enumerate(lengths)]
     g = [x.clone() for x in before]
     out = None if out_dtype is None else [torch.empty(n, device=DEV, dtype=out_dtype) for n in lengths]
     want = exact_norm(before, kind)
     max_norm = 0.37 * want + 1e-3 * (want == 0)
-    norm = ops.clip_grads(g, max_norm, norm_type=kind, out=out)
+    norm = ops.clip_grads(ops.TensorTable(g, out=out), max_norm, norm_type=kind) if kept else ops.clip_grads(g, max_norm, norm_type=kind, out=out)
     check_norm(norm, before, kind)
     for x, b, o in zip(g, before, g if out is None else out):
         check_clipped(o, b, coefficient(want, max_norm))
@@ -271,13 +274,14 @@ COMBOS = [(F32, F32), (F32, BF16), (F32, F16), (BF16, BF16), (BF16, F32), (F16, 
 
 
 @pytest.mark.parametrize("pt,gt", COMBOS, ids=str)
-@pytest.mark.parametrize("lengths", [[1], [255, 0, 257], [16385], [5] * 150, [1023, 70001, 2]], ids=lambda v: f"{len(v)}x{max(v)}")
+@pytest.mark.parametrize("lengths", [[1], [255, 0, 257], [16385], [5] * 150, [1023, 70001, 2], [4_500_001], [17_000_003, 5]], ids=lambda v: f"{len(v)}x{max(v)}")
+@pytest.mark.parametrize("kept", [False, True])
 @pytest.mark.parametrize("clip,decay,offset", [(None, 0.0, 0), (0.5, 0.1, 0), (1e9, 0.01, 1), (0.3, 0.0, 3)])
-def test_adam(lengths, pt, gt, clip, decay, offset):
+def test_adam(lengths, pt, gt, clip, decay, offset, kept):
     s = adam_state(lengths, pt, gt, offset=offset)
     before = copy_state(s)
     lr, step = 1e-2, 7
-    norm = ops.adam_step_tensors([s], lr=lr, step=step, weight_decay=decay, max_norm=clip)
+    norm = ops.adam_step_tensors(ops.AdamTable([s]) if kept else [s], lr=lr, step=step, weight_decay=decay, max_norm=clip)
     if clip is None:
         assert norm is None
     else:

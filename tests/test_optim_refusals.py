@@ -79,6 +79,34 @@ def test_c_table_counts_what_it_holds():
     assert grad_table([(1024, 2048, 1 << 44, 0, 0)] * 3, 0)[0] == -1 and "chunks" in err()
 
 
+@pytest.mark.parametrize("lengths", [[1], [4096], [4097], [530052, 530052, 165900, 2304], [5] * 3000, [100000] * 100, [1 << 20] * 5, [1 << 20] * 16, [3, 7]])
+@pytest.mark.parametrize("offset", [0, 2, 126])
+def test_c_kept_tables_cut_small_lists_into_pieces(lengths, offset):
+    """the image of a kept table holds every element of every tensor once, in order, and fits the size that was asked for"""
+    lib = _lib.load()
+    rows, at = [], (1 << 30) + offset
+    for n in lengths:
+        rows.append((at, at, n, 1, 1))
+        at += 2 * n + 64
+    image, t = ctypes.create_string_buffer(lib.niw_table_bytes(len(rows))), _lib.Table()
+    assert lib.niw_grad_table(grads(*rows), len(rows), 3, image, ctypes.byref(t)) == 0
+    assert t.bytes <= len(image) and t.slots >= len(rows)
+    slots = [(int.from_bytes(image.raw[32 * i:32 * i + 8], "little"), int.from_bytes(image.raw[32 * i + 16:32 * i + 24], "little"),
+              int.from_bytes(image.raw[32 * i + 24:32 * i + 28], "little")) for i in range(t.slots)]
+    k, chunks = 0, 0
+    for begin, _, n, _, _ in rows:
+        here = begin
+        while here < begin + 2 * n:
+            assert slots[k][0] == here and slots[k][2] == chunks
+            here += 2 * slots[k][1]
+            chunks += -(-slots[k][1] // t.chunk)
+            k += 1
+        assert here == begin + 2 * n
+    assert k == t.slots and chunks == t.chunks
+    first = [int.from_bytes(image.raw[32 * t.slots + 4 * i:32 * t.slots + 4 * i + 4], "little") for i in range(t.slots)]
+    assert first == [s[2] for s in slots]
+
+
 def test_c_calls_refuse_bad_arguments():
     lib = _lib.load()
     t = grad_table([(1024, 1024, 4, 0, 0)], 1)[1]
@@ -89,6 +117,8 @@ def test_c_calls_refuse_bad_arguments():
     assert lib.niw_grad_table(None, 1, 0, 4096, R(_lib.Table())) == -1 and "1 tensors" in err()
     assert lib.niw_grad_table(None, -1, 0, 4096, R(_lib.Table())) == -1 and "-1 tensors" in err()
     assert lib.niw_grad_table(grads((1024, 1024, 4, 0, 0)), 1, 0, None, R(_lib.Table())) == -1 and "null pointer" in err()
+    assert lib.niw_grad_table(grads((1024, 1024, 4, 0, 0)), 1, 4, 4096, R(_lib.Table())) == -1 and "flags 4" in err()
+    assert lib.niw_adam_table(adam_row(), 1, 1, 1, 4096, R(_lib.Table())) == -1 and "flags 1" in err()
     assert lib.niw_table_bytes(-1) == 0
     assert lib.niw_table_store(None, 16, 4096, None) == -1 and "null" in err()
     assert lib.niw_table_store(4096, 16, 4097, None) == -1 and "misaligned" in err()
@@ -120,7 +150,7 @@ def adam_row(**kw):
 def adam_table(n_groups=1, **kw):
     lib = _lib.load()
     image, t = ctypes.create_string_buffer(lib.niw_table_bytes(1)), _lib.Table()
-    return lib.niw_adam_table(adam_row(**kw), 1, n_groups, image, ctypes.byref(t)), t
+    return lib.niw_adam_table(adam_row(**kw), 1, n_groups, 0, image, ctypes.byref(t)), t
 
 
 @pytest.mark.parametrize("change,what", [
