@@ -6,6 +6,7 @@ import ctypes
 import contextlib
 import math
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -309,21 +310,46 @@ def _check_dense(t, name):
         run *= n
 
 
-def _check_same_layout(a, b, name):
-    if a.shape != b.shape or (_layout(a) != _layout(b) and a.numel() > 1):
-        raise _lib.NiwError(f"{name}: shape {tuple(b.shape)} strides {b.stride()} against {tuple(a.shape)} {a.stride()}; the elements of a pair have to "
-                            "lie in the same order")
+def _check_all(tensors, name):
+    """_check_dense of a list whose tensors are nearly always plain: a quick look at all of them first"""
+    if not all(isinstance(t, torch.Tensor) and t.dtype in DTYPES and t.layout is torch.strided and t.is_contiguous() and not t.is_neg() for t in tensors):
+        for i, t in enumerate(tensors):
+            _check_dense(t, f"{name} {i}")
+
+
+def _check_pairs(first, second, name):
+    """the elements of a pair lie in the same order: both contiguous (of whatever shapes), or laid out alike"""
+    for i, (a, b) in enumerate(zip(first, second)):
+        if a.numel() != b.numel() or not (a.is_contiguous() and b.is_contiguous() or a.numel() < 2 or (a.shape == b.shape and _layout(a) == _layout(b))):
+            raise _lib.NiwError(f"{name} {i}: shape {tuple(b.shape)} strides {b.stride()} against {tuple(a.shape)} {a.stride()}; the elements of a pair have to "
+                                "lie in the same order")
 
 
 def _check_device(tensors, name):
     """the one GPU all of them are on (None: an empty list)"""
-    devices = {t.device for t in tensors}
-    if len(devices) > 1:
-        raise _lib.NiwError(f"{name}: tensors on several devices ({', '.join(sorted(map(str, devices)))})")
-    device = devices.pop() if devices else None
-    if device is not None and device.type != "cuda":
+    if not tensors:
+        return None
+    device = tensors[0].device
+    if any(t.get_device() != device.index if device.type == "cuda" else True for t in tensors):
+        devices = {t.device for t in tensors}
+        if len(devices) > 1:
+            raise _lib.NiwError(f"{name}: tensors on several devices ({', '.join(sorted(map(str, devices)))})")
         raise _lib.NiwError(f"{name}: expected CUDA/HIP tensors, got {device}")
     return device
+
+
+# rows of niw_grad_tensor / niw_adam_tensor (include/niw.h); a list's are filled column by column
+_GRAD_ROW = np.dtype([("grad", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("out_dtype", "<i4")])
+_ADAM_ROW = np.dtype([("param", "<u8"), ("grad", "<u8"), ("exp_avg", "<u8"), ("exp_avg_sq", "<u8"), ("master", "<u8"), ("n", "<i8"), ("param_dtype", "<i4"),
+                      ("grad_dtype", "<i4"), ("group", "<i4"), ("reserved", "<i4")])
+
+
+def _addresses(tensors):
+    return [t.data_ptr() for t in tensors]
+
+
+def _types(tensors):
+    return [DTYPES[t.dtype] for t in tensors]
 
 
 def _on(device):
@@ -337,12 +363,13 @@ class _Table:
     """Device image of a list of tensors (niw_table).  The image is stored on the stream that is current when the table is built; a table that
     is kept (`kept`) waits for that once, so that any stream may use it afterwards."""
 
-    def _build(self, name, entries, how, tensors, kept):
+    def _build(self, name, rows, how, tensors, kept):
         lib = _lib.load()
-        self._keep = [(t, t.untyped_storage()) for t in tensors]
-        host = ctypes.create_string_buffer(max(lib.niw_table_bytes(len(entries)), 16))
+        self._keep = [tensors, [t.untyped_storage() for t in tensors]]
+        host = np.empty(max(lib.niw_table_bytes(len(rows)), 16), np.uint8)
+        image = ctypes.c_void_p(host.ctypes.data)
         self._c = _lib.Table()
-        if getattr(lib, name)(entries, len(entries), *how, host, ctypes.byref(self._c)):
+        if getattr(lib, name)(ctypes.c_void_p(rows.ctypes.data), len(rows), *how, image, ctypes.byref(self._c)):
             raise _lib.NiwError(lib.niw_last_error_string().decode())
         self._stream, self._image = None, None
         if self._c.bytes:
@@ -352,7 +379,7 @@ class _Table:
                 self._image = torch.empty(self._c.bytes, device=self.device, dtype=torch.uint8)
                 self._c.image = self._image.data_ptr()
                 stream = torch.cuda.current_stream()
-                _lib.call("niw_table_store", host, self._c.bytes, _p(self._image), ctypes.c_void_p(stream.cuda_stream))
+                _lib.call("niw_table_store", image, self._c.bytes, _p(self._image), ctypes.c_void_p(stream.cuda_stream))
                 self._stream = stream.cuda_stream
                 if kept:
                     stream.synchronize()
@@ -370,7 +397,8 @@ class TensorTable(_Table):
     """What grad_norm / grad_total / clip_grads need to know of a list of tensors, gathered and checked once for tensors that stay where they
     are (a gradient bucket's views, gradients that are zeroed rather than dropped).  A plain list in its place is gathered at every call.
     tensors: float32 / bfloat16 / float16, mixed at will, each dense in any order, any length; None entries are left out.
-    out: for clip_grads, one tensor per entry that receives the clipped values (same shape and order, any of the types); None: in place.
+    out: for clip_grads, one tensor per entry that receives the clipped values, of any of the types (as many elements in the same order: both
+    contiguous, of whatever shapes, or laid out alike); None: in place.
     The table speaks of the MEMORY the tensors had when it was built and keeps that memory alive; a tensor that is given other storage
     afterwards (.grad re-created by a backward, .data re-assigned, .to()) is not followed: build a new table.  Building one waits for the GPU
     once; any stream, thread or captured graph may use it then, several at a time (a graph does not keep it alive: the caller does)."""
@@ -380,29 +408,33 @@ class TensorTable(_Table):
         out = [None] * len(tensors) if out is None else list(out)
         if len(out) != len(tensors):
             raise _lib.NiwError(f"TensorTable: {len(tensors)} tensors and {len(out)} outputs")
-        pairs = [(t, o) for t, o in zip(tensors, out) if t is not None]
-        if len({o is None for _, o in pairs}) > 1:
+        keep = [i for i, t in enumerate(tensors) if t is not None]
+        if len(keep) < len(tensors):
+            tensors, out = [tensors[i] for i in keep], [out[i] for i in keep]
+        given = sum(o is not None for o in out)
+        if given not in (0, len(out)):
             raise _lib.NiwError("TensorTable: an output for some tensors only")
-        for i, (t, o) in enumerate(pairs):
-            _check_dense(t, f"tensor {i}")
-            if o is not None:
-                _check_dense(o, f"output {i}")
-                _check_same_layout(t, o, f"output {i}")
-        every = [x for p in pairs for x in p if x is not None]
+        _check_all(tensors, "tensor")
+        if given:
+            _check_all(out, "output")
+            _check_pairs(tensors, out, "output")
+        else:
+            out = tensors
+        every = tensors + out if given else tensors
         self.device = _check_device(every, "TensorTable")
-        self.numel = sum(t.numel() for t, _ in pairs)
-        entries = (_lib.GradTensor * len(pairs))()
-        for c, (t, o) in zip(entries, pairs):
-            o = t if o is None else o
-            c.grad, c.out, c.n, c.dtype, c.out_dtype = t.data_ptr(), o.data_ptr(), t.numel(), DTYPES[t.dtype], DTYPES[o.dtype]
+        rows = np.zeros(len(tensors), _GRAD_ROW)
+        rows["grad"], rows["out"], rows["n"] = _addresses(tensors), _addresses(out), [t.numel() for t in tensors]
+        rows["dtype"], rows["out_dtype"] = _types(tensors), _types(out)
+        self.numel = int(rows["n"].sum())
+        kept = TABLE_KEPT if _kept else 0
         self._unclippable = None
         try:
-            self._build("niw_grad_table", entries, (TABLE_CLIP | (TABLE_KEPT if _kept else 0),), every, _kept)
+            self._build("niw_grad_table", rows, (TABLE_CLIP | kept,), every, _kept)
         except _lib.NiwError as e:
-            if pairs[0][1] is not None or "overlap" not in str(e):
+            if given or "overlap" not in str(e):
                 raise
             self._unclippable = str(e)               # tensors that share memory have a norm, but cannot be clipped in place
-            self._build("niw_grad_table", entries, (TABLE_KEPT if _kept else 0,), every, _kept)
+            self._build("niw_grad_table", rows, (kept,), every, _kept)
 
 
 def _table(grads, out=None):
@@ -484,49 +516,53 @@ class AdamTable(_Table):
         grads       float32 / bfloat16 / float16; a None entry leaves its parameter out
         exp_avg, exp_avg_sq     float32
         master      float32 copies that the update runs on (half-precision parameters receive the rounded result), None for float32
-    The tensors of one entry have the same shape and the same order in memory."""
+    The tensors of one entry have as many elements in the same order in memory (all contiguous, of whatever shapes, or laid out alike)."""
 
     def __init__(self, groups, _kept=True):
         groups = [dict(g) for g in groups]
         if not 1 <= len(groups) <= 8:
             raise _lib.NiwError(f"AdamTable: 1..8 groups (got {len(groups)})")
-        rows = []
+        names = ("params", "grads", "exp_avg", "exp_avg_sq")
+        cols, master, group = {key: [] for key in names}, [], []
         for k, g in enumerate(groups):
-            lists = {key: g.pop(key, None) for key in ("params", "grads", "exp_avg", "exp_avg_sq", "master")}
+            lists = {key: g.pop(key, None) for key in names + ("master",)}
             if g:
                 raise _lib.NiwError(f"AdamTable: group {k} has unknown keys {sorted(g)}")
-            lists = {key: None if v is None else list(v) for key, v in lists.items()}
-            if any(lists[key] is None for key in ("params", "grads", "exp_avg", "exp_avg_sq")):
+            if any(lists[key] is None for key in names):
                 raise _lib.NiwError(f"AdamTable: group {k} needs params, grads, exp_avg and exp_avg_sq")
             n = len(lists["params"])
-            if any(v is not None and len(v) != n for v in lists.values()):
+            lists["master"] = [None] * n if lists["master"] is None else lists["master"]
+            if any(len(v) != n for v in lists.values()):
                 raise _lib.NiwError(f"AdamTable: the lists of group {k} differ in length")
-            for i in range(n):
-                row = {key: None if v is None else v[i] for key, v in lists.items()}
-                if row["grads"] is None:
-                    continue
-                name = f"group {k} entry {i}"
-                for key, t in row.items():
-                    if t is None and key == "master":
-                        continue
-                    _check_dense(t, f"{name} {key}")
-                    if key not in ("params", "grads") and t.dtype != torch.float32:
-                        raise _lib.NiwError(f"{name} {key}: expected float32, got {t.dtype}")
-                    _check_same_layout(row["params"], t, f"{name} {key}")
-                if (row["params"].dtype == torch.float32) != (row["master"] is None):
-                    raise _lib.NiwError(f"{name}: a half-precision parameter needs a float32 master copy (updates below half a step of its type would be "
-                                        "lost), a float32 parameter has none")
-                rows.append((k, row))
-        tensors = [t for _, row in rows for t in row.values() if t is not None]
+            keep = [i for i, t in enumerate(lists["grads"]) if t is not None]
+            for key in names:
+                cols[key] += [lists[key][i] for i in keep]
+            master += [lists["master"][i] for i in keep]
+            group += [k] * len(keep)
+        masters = [t for t in master if t is not None]
+        for key in names:
+            _check_all(cols[key], key)
+        _check_all(masters, "master")
+        for key, t in [(key, t) for key in names[2:] for t in cols[key]] + [("master", t) for t in masters]:
+            if t.dtype != torch.float32:
+                raise _lib.NiwError(f"AdamTable: {key}: expected float32, got {t.dtype}")
+        for p, w in zip(cols["params"], master):
+            if (p.dtype == torch.float32) != (w is None):
+                raise _lib.NiwError("AdamTable: a half-precision parameter needs a float32 master copy (updates below half a step of its type would be "
+                                    "lost), a float32 parameter has none")
+        for key in names[1:]:
+            _check_pairs(cols["params"], cols[key], key)
+        _check_pairs([p for p, w in zip(cols["params"], master) if w is not None], masters, "master")
+        tensors = [t for key in names for t in cols[key]] + masters
         self.device = _check_device(tensors, "AdamTable")
         self.n_groups = len(groups)
-        self.numel = sum(row["params"].numel() for _, row in rows)
-        entries = (_lib.AdamTensor * len(rows))()
-        for c, (k, row) in zip(entries, rows):
-            c.param, c.grad, c.exp_avg, c.exp_avg_sq = (row[key].data_ptr() for key in ("params", "grads", "exp_avg", "exp_avg_sq"))
-            c.master = None if row["master"] is None else row["master"].data_ptr()
-            c.n, c.param_dtype, c.grad_dtype, c.group = row["params"].numel(), DTYPES[row["params"].dtype], DTYPES[row["grads"].dtype], k
-        self._build("niw_adam_table", entries, (self.n_groups, TABLE_KEPT if _kept else 0), tensors, _kept)
+        rows = np.zeros(len(group), _ADAM_ROW)
+        for field, key in zip(("param", "grad", "exp_avg", "exp_avg_sq"), names):
+            rows[field] = _addresses(cols[key])
+        rows["master"], rows["n"], rows["group"] = [0 if w is None else w.data_ptr() for w in master], [p.numel() for p in cols["params"]], group
+        rows["param_dtype"], rows["grad_dtype"] = _types(cols["params"]), _types(cols["grads"])
+        self.numel = int(rows["n"].sum())
+        self._build("niw_adam_table", rows, (self.n_groups, TABLE_KEPT if _kept else 0), tensors, _kept)
 
 
 def _per_group(value, n, name, kind):

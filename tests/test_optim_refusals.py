@@ -211,6 +211,13 @@ def test_tensor_table_refuses(tensors, out, what):
         ops.TensorTable(tensors, out=out)
 
 
+def test_rows_of_a_list_have_the_layout_of_the_descriptors():
+    """the columns the wrappers fill are the fields of include/niw.h"""
+    for row, struct in ((ops._GRAD_ROW, _lib.GradTensor), (ops._ADAM_ROW, _lib.AdamTensor)):
+        assert row.itemsize == ctypes.sizeof(struct)
+        assert [(n, row.fields[n][1]) for n in row.names] == [(n, getattr(struct, n).offset) for n, _ in struct._fields_]
+
+
 def test_none_entries_are_left_out_before_any_check():
     with pytest.raises(_lib.NiwError, match="expected CUDA/HIP"):
         ops.TensorTable([None, z(4)], out=[None, z(4)])
@@ -239,7 +246,7 @@ def group(**kw):
     ([], "1..8 groups"), ([group()] * 9, "1..8 groups"),
     ([group(lr=[1.0])], "unknown keys"), ([group(grads=None)], "needs params"), ([group(grads=[])], "differ in length"),
     ([group(exp_avg=[z(4, dtype=torch.bfloat16)])], "expected float32"), ([group(params=[z(4, dtype=torch.bfloat16)])], "master copy"),
-    ([group(master=[z(4)])], "has none"), ([group(grads=[z(2, 2)])], "same order"),
+    ([group(master=[z(4)])], "has none"), ([group(grads=[z(5)])], "same order"),
     ([group(params=[z(2, 3)], grads=[z(3, 2).t()], exp_avg=[z(2, 3)], exp_avg_sq=[z(2, 3)])], "same order"),
     ([group(params=[z(8)[::2]])], "gaps"), ([group()], "expected CUDA/HIP"), ([group(grads=[z(4, dtype=torch.float64)])], "float64"),
 ])
