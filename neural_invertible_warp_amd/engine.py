@@ -3,8 +3,8 @@
 model/base.py:130-142):
 
     zero_grad -> graph.forward(mode="train", iter=it) -> compute_loss -> summarize_loss (sum of 10^w * loss)
-    -> backward -> Adam(nerf[, nerf_fine]) + Adam(warp network, latent table) -> ExponentialLR -> it += 1
-    -> progress = it / max_iter
+    -> backward -> [clip by the global gradient norm, optim.clip_norm] -> Adam(nerf[, nerf_fine]) + Adam(warp network, latent table)
+    -> ExponentialLR -> it += 1 -> progress = it / max_iter
 
 The Adam updates run as fused launches over flat buffers (niw_adam_step); under ray sharding the gradients of all
 groups are summed over ranks in ONE flat all-reduce first (..parallel.GradBucket).  Two model families share it:
@@ -343,6 +343,47 @@ class FusedStep:
         return loss
 
 
+def clip_options(optim):
+    """-> (optim.clip_norm as a float or None, optim.skip_nonfinite)"""
+    max_norm, skip = optim.get("clip_norm"), bool(optim.get("skip_nonfinite"))
+    if max_norm is None:
+        if skip:
+            raise NiwError("optim.skip_nonfinite goes with optim.clip_norm (.inf clips nothing)")
+        return None, False
+    try:
+        value = math.nan if isinstance(max_norm, bool) else float(max_norm)      # (yaml reads 1e-3 as text)
+    except (TypeError, ValueError):
+        value = math.nan
+    if not value >= 0.0:
+        raise NiwError(f"optim.clip_norm={max_norm!r}: a number from 0 on (.inf clips nothing)")
+    return value, skip
+
+
+class ClippedAdam:
+    """The optimizer step of a trainer under `optim.clip_norm` (ops.adam_step_tensors): the gradients of all trained groups are scaled by
+    min(1, clip_norm / (norm + 1e-6)), norm = the global norm over all of them, inside the Adam launch.  One launch for the norm, one for the update.
+    Under ray sharding the step comes behind the gradient exchange: every rank forms the same norm of the same sums.
+    `norm` afterwards: the norm of the last step (0-d device tensor; under graph replay the graph's own, read it before the next step).
+    `optim.skip_nonfinite`: a step whose norm is not finite changes nothing (the schedule and the step number go on)."""
+
+    def __init__(self, optim):
+        self.max_norm, self.skip_nonfinite = clip_options(optim)
+        self.norm, self._table, self._addresses = None, None, None
+
+    def table(self, rows):
+        """rows: (param, grad, exp_avg, exp_avg_sq) flat buffers per group, None for a group that is not trained (it keeps its place).  The launch
+        table is built again when a buffer has moved."""
+        addresses = [None if r is None else tuple(t.data_ptr() for t in r) for r in rows]
+        if addresses != self._addresses:
+            part = lambda r, k: [] if r is None else [r[k]]
+            self._table = ops.AdamTable([dict(params=part(r, 0), grads=part(r, 1), exp_avg=part(r, 2), exp_avg_sq=part(r, 3)) for r in rows])
+            self._addresses = addresses
+        return self._table
+
+    def step(self, rows, lr, step, hyper_dev=None):
+        self.norm = ops.adam_step_tensors(self.table(rows), lr=lr, step=step, max_norm=self.max_norm, skip_nonfinite=self.skip_nonfinite, hyper_dev=hyper_dev)
+
+
 class INNTrainer:
     def __init__(self, opt, n_views, rank=0, world=1, warp_perturb=0.0, seed=0, initial_poses_w2c=None, ray_sampler=None, hip_graph=False,
                  fused_step="auto", overlap=True, split_exchange="auto", collectives=True):
@@ -363,6 +404,7 @@ class INNTrainer:
         o = opt.optim
         if o.get("algo", "Adam") != "Adam":
             raise NiwError(f"optim.algo={o.algo!r}: only Adam is fused (niw_adam_step)")
+        self.clip = ClippedAdam(o)
         torch.manual_seed(seed)                       # identical initial weights on every rank
         self.family = "dtu" if opt.model == "barf_inn_dtu" else "llff"
         if self.family == "dtu":
@@ -624,10 +666,22 @@ class INNTrainer:
 
     def _optimizer_step(self, it):
         """torch.optim.Adam's update of every trained group (reference nerf.py:34-38, barf_inn_llff.py:84-104: two optimizers stepped one
-        after the other) as ONE launch over the flat buffers"""
+        after the other) as ONE launch over the flat buffers; under optim.clip_norm see ClippedAdam"""
+        if self.clip.max_norm is not None:
+            self.clip.step(self._clip_rows(), [self.learning_rate(i, it) for i in range(len(self.bucket.groups))], it + 1,
+                           hyper_dev=self.consts.hyper_all if self.hip_graph else None)
+            return
         groups = [(flat, self.bucket.segment(i), self.m[i], self.v[i], self.learning_rate(i, it), it + 1) if self.trainable[i] else None
                   for i, flat in enumerate(self._flats())]
         ops.adam_step_multi(groups, hyper_dev=self.consts.hyper_all if self.hip_graph else None)
+
+    def _clip_rows(self):
+        return [(flat, self.bucket.segment(i), self.m[i], self.v[i]) if self.trainable[i] else None for i, flat in enumerate(self._flats())]
+
+    @property
+    def grad_norm(self):
+        """global gradient norm of the last iteration (0-d device tensor) under optim.clip_norm, else None"""
+        return self.clip.norm
 
     def _upload_constants(self, it):
         """the scalars of 0-based iteration `it` (progress it / max_iter was set after the previous step, barf_inn_llff.py:117)"""
@@ -688,7 +742,7 @@ class INNTrainer:
             # graph would read and write the old storage -- record the iteration again instead
             self._captured = None
             return self._graph_iteration(var, it, replay)
-        fb, adam, loss = self._captured
+        fb, adam, loss, self.clip.norm = self._captured
         fb.replay()
         if adam is not None:                           # ranks exchange gradients between the two graphs
             self._all_reduce()
@@ -738,6 +792,8 @@ class INNTrainer:
         import sys
         import torch.distributed as dist
         live_group = parallel._collectives_live()
+        if self.clip.max_norm is not None:
+            self.clip.table(self._clip_rows())      # (built in front of the capture: storing it waits for the GPU)
         # (round 3: no collective sits inside the forward any more -- the warp and the alignment term are replicated, ..parallel --
         # so a sharded iteration is captured like any other: forward + backward + gather | all-reduce, eager | Adam)
         torch.cuda.synchronize()                    # (`var` holds the trainer's own copies of the batch: the graph reads them in place)
@@ -773,7 +829,7 @@ class INNTrainer:
         finally:
             if gc_was_on:
                 gc.enable()
-        self._captured = (fb, adam, loss)
+        self._captured = (fb, adam, loss, self.clip.norm)
         self._captured_addresses = self._capture_addresses()
         return True
 
@@ -837,6 +893,7 @@ class NeRFTrainer:
         o = opt.optim
         self.lr0, self.gamma = o.lr, _sched_gamma(o.lr, o.get("lr_end"), o.get("sched", {"type": "ExponentialLR"}), opt.max_iter, "optim.sched")
         n = len(self.nets)
+        self.clip = ClippedAdam(o)
         self.lrs, self.gammas, self.trainable = [(o.lr, o.get("lr_end"))] * n, [self.gamma] * n, [True] * n          # (checkpoint.py reads these)
         on_gpu = dev.type == "cuda"
         opt.nerf.ray_sampler = opt.nerf.get("ray_sampler") or ("feistel" if on_gpu else "randperm")
@@ -885,12 +942,20 @@ class NeRFTrainer:
             torch.autograd.backward([loss[k] for k in keys], [torch.full_like(loss[k], 10 ** float(opt.loss_weight[k])) for k in keys])
             loss.update(all=total)
         lr = self.lr0 * self.gamma ** it
-        ops.adam_step_multi([(n_.flat_params, self.bucket.segment(i), self.m[i], self.v[i], lr, it + 1) for i, n_ in enumerate(self.nets)])
+        if self.clip.max_norm is not None:
+            self.clip.step([(n_.flat_params, self.bucket.segment(i), self.m[i], self.v[i]) for i, n_ in enumerate(self.nets)], lr, it + 1)
+        else:
+            ops.adam_step_multi([(n_.flat_params, self.bucket.segment(i), self.m[i], self.v[i], lr, it + 1) for i, n_ in enumerate(self.nets)])
         self.it = it + 1
         return loss
 
     def _flats(self):
         return [n.flat_params for n in self.nets]
+
+    @property
+    def grad_norm(self):
+        """global gradient norm of the last iteration (0-d device tensor) under optim.clip_norm, else None"""
+        return self.clip.norm
 
 
 def synthetic_scene(opt, n_views, seed=0):

@@ -107,6 +107,7 @@ class Model(_nerf.Model):
         var = self.graph.forward(opt, edict(var), mode="train", iter=self.it)
         loss = self.summarize_loss(opt, var, self.graph.compute_loss(opt, var, mode="train"))
         loss.all.backward()
+        self._clip(self.optim, self.optim_pose)
         self.optim.step()
         self.optim_pose.step()
         self.sched_pose.step()

@@ -162,7 +162,9 @@ class Model:
         return self.trainer.summarize_loss(loss)
 
     def log_scalars(self, opt, var, loss, metric=None, step=0, split="train"):
-        msg = " ".join("{}={:.5f}".format(k, float(torch.as_tensor(v).detach())) for k, v in loss.items())
+        norm = self.trainer.grad_norm if split == "train" else None
+        scalars = list(loss.items()) + ([] if norm is None else [("grad_norm", norm)])
+        msg = " ".join("{}={:.5f}".format(k, float(torch.as_tensor(v).detach())) for k, v in scalars)
         print("[{} it {}] {}".format(split, step, msg), flush=True)
 
     def _evaluator(self, opt):

@@ -391,6 +391,7 @@ class Model:
     reference builds them (the parameters are ordinary nn.Parameters, views of the flat buffers the kernels read).  Checkpoints are
     the reference's model.ckpt dict either way (graph, optim, sched, epoch, iter).  Logging back-ends are outside the path."""
 
+    grad_norm = None      # torch.optim path under optim.clip_norm: global gradient norm of the last iteration (0-d device tensor)
     trainer = None        # engine.NeRFTrainer when build_networks chose the engine (subclasses that build their own graph keep the torch path)
 
     def __init__(self, opt):
@@ -420,6 +421,10 @@ class Model:
     def setup_optimizer(self, opt):
         if self.trainer is not None:
             return                                    # the trainer owns the flat Adam state and the ExponentialLR schedule
+        from .. import engine
+        self.clip_norm, skip = engine.clip_options(opt.optim)
+        if skip:
+            raise NiwError(f"optim.skip_nonfinite: the fused Adam step leaves a step out, optim.algo={opt.optim.algo} does not")
         optimizer = getattr(torch.optim, opt.optim.algo)
         self.optim = optimizer([dict(params=self.graph.nerf.parameters(), lr=opt.optim.lr)])
         if opt.nerf.fine_sampling:
@@ -470,7 +475,9 @@ class Model:
             if self.trainer is None:
                 self.sched.step()
             if self.it % opt.freq.scalar == 0:
-                print("[train it {}] {}".format(self.it, " ".join("{}={:.5f}".format(k, float(v.detach())) for k, v in loss.items())), flush=True)
+                norm = self.grad_norm if self.trainer is None else self.trainer.grad_norm
+                scalars = list(loss.items()) + ([] if norm is None else [("grad_norm", norm)])
+                print("[train it {}] {}".format(self.it, " ".join("{}={:.5f}".format(k, float(v.detach())) for k, v in scalars)), flush=True)
             if self.it % opt.freq.val == 0:
                 self.validate(opt, self.it)
             if self.it % opt.freq.ckpt == 0:
@@ -494,9 +501,15 @@ class Model:
         var = self.graph.forward(opt, edict(var), mode="train")
         loss = self.summarize_loss(opt, var, self.graph.compute_loss(opt, var, mode="train"))
         loss.all.backward()
+        self._clip(self.optim)
         self.optim.step()
         self.it += 1
         return loss
+
+    def _clip(self, *optimizers):
+        """optim.clip_norm on the torch.optim path: the gradients of all parameters of the optimizers, clipped in place by their global norm"""
+        if self.clip_norm is not None:
+            self.grad_norm = ops.clip_grads([p.grad for o in optimizers for g in o.param_groups for p in g["params"]], self.clip_norm)
 
     @torch.no_grad()
     def validate(self, opt, ep=None):

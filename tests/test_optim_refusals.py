@@ -264,3 +264,27 @@ def test_adam_step_tensors_refuses(kw, what):
     empty = ops.AdamTable([dict(params=[], grads=[], exp_avg=[], exp_avg_sq=[])])
     with pytest.raises(_lib.NiwError, match=what):
         ops.adam_step_tensors(empty, **{**dict(lr=1e-3, step=1), **kw})
+
+
+@pytest.mark.parametrize("optim,what", [
+    (dict(clip_norm=-1.0), "from 0 on"), (dict(clip_norm=float("nan")), "from 0 on"), (dict(clip_norm=True), "from 0 on"), (dict(clip_norm="much"), "from 0 on"), (dict(clip_norm=[1]), "from 0 on"),
+    (dict(skip_nonfinite=True), "goes with optim.clip_norm"),
+])
+def test_trainer_options_are_checked(optim, what):
+    from neural_invertible_warp_amd import engine
+    with pytest.raises(_lib.NiwError, match=what):
+        engine.ClippedAdam(optim)
+
+
+def test_trainer_without_the_option_has_no_clip():
+    from neural_invertible_warp_amd import engine
+    assert engine.ClippedAdam({}).max_norm is None and engine.ClippedAdam(dict(clip_norm=0)).max_norm == 0.0
+    assert engine.clip_options(dict(clip_norm="1e-3", skip_nonfinite=True)) == (1e-3, True)      # as the command line's yaml reads it
+
+
+def test_torch_optimizers_refuse_to_leave_a_step_out():
+    from neural_invertible_warp_amd.model import nerf
+    from neural_invertible_warp_amd.util import edict
+    m = nerf.Model.__new__(nerf.Model)
+    with pytest.raises(_lib.NiwError, match="does not"):
+        m.setup_optimizer(edict(optim=edict(algo="AdamW", lr=1e-3, clip_norm=1.0, skip_nonfinite=True)))
