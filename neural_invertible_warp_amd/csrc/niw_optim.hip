@@ -44,6 +44,9 @@ static_assert(kNormBlocks <= NIW_NORM_WORKSPACE_DOUBLES - 1, "a partial sum per 
 constexpr int kAdamPart = 1024;
 constexpr int kClipPart = 4096, kClipPartWide = 2048;      // (wide: fp32 to fp32, 8 bytes per element; in place 933 us against 963 for 2 GB,
                                                            // but bf16 to fp32 461 against 423 for 335 M)
+// Parts in a row per die (part_of): 256 KB of an fp32 stream.  Adam of 335 M bf16 parameters 1.69 -> 1.58 ms (16 parts 1.64, 32 1.59, 128
+// 1.68), 2 GB clipped in place 950 -> 927 us; bf16 to fp32 gains nothing (424 to 447 us with any).
+constexpr int kAdamStretch = 64, kClipStretchWide = 32;
 // The workgroups of a clip or an update join the norm's partial sums themselves as long as they are few (kFoldGrid): saves a launch,
 // 3 us of the trainer's 18; with 120,000 workgroups one more launch is cheaper (2 GB in place: 963 us against 973).
 constexpr int kFoldGrid = 4096;
@@ -165,9 +168,14 @@ struct Part {
     int head;
     bool any;
 };
-template <int PART, class Slot>
+template <int PART, int STRETCH, class Slot>
 __device__ __forceinline__ Part<Slot> part_of(const List<Slot>& list) {
-    const int split = parts_of(list, PART), b = (int)blockIdx.x / split, part = split - 1 - (int)blockIdx.x % split;
+    // workgroups go to the eight dies in turn: of every 8 x STRETCH parts each die takes STRETCH that follow each other
+    constexpr unsigned kDies = 8, kGroup = kDies * STRETCH;
+    unsigned at_grid = blockIdx.x;
+    const unsigned group = at_grid / kGroup * kGroup;
+    if (STRETCH > 1 && group + kGroup <= gridDim.x) at_grid = group + at_grid % kDies * STRETCH + (at_grid - group) / kDies;
+    const int split = parts_of(list, PART), b = (int)at_grid / split, part = split - 1 - (int)at_grid % split;
     const int c = list.chunks - 1 - b;
     Part<Slot> p{};
     if (c < 0) return p;
@@ -369,7 +377,7 @@ __device__ __forceinline__ Factor clip_factor(const Clip& clip) {
 template <int KIND, bool NT, int PART>
 __global__ __launch_bounds__(kThreads) void clip_kernel(List<GradSlot> list, Clip clip) {
     const float c = clip_factor<KIND>(clip).c;
-    const auto part = part_of<PART>(list);
+    const auto part = part_of<PART, PART == kClipPartWide ? kClipStretchWide : 1>(list);
     const GradSlot& s = part.s;
     if (!part.any || (c == 1.f && s.o == s.g)) return;
     with_dtype(s.types & 255, [&](auto gt) {
@@ -401,7 +409,7 @@ struct AdamArgs {
 template <int KIND, bool NT>
 __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> list, AdamArgs a, Clip clip) {
     const Factor factor = clip_factor<KIND>(clip);
-    const auto part = part_of<kAdamPart>(list);
+    const auto part = part_of<kAdamPart, kAdamStretch>(list);
     if (!part.any || factor.skip) return;
     const AdamSlot& s = part.s;
     const int k = __builtin_amdgcn_readfirstlane(s.types >> 16), tid = threadIdx.x;
