@@ -465,7 +465,11 @@ __global__ __launch_bounds__(kThreads) void store_kernel(Piece piece, u32x4* __r
 bool known(int dtype) { return dtype == NIW_F32 || dtype == NIW_BF16 || dtype == NIW_F16; }
 bool aligned(const void* p, int size) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(size - 1)) == 0; }
 constexpr int64_t kMaxElements = 1ll << 44, kMaxTensors = 1ll << 20;
-constexpr int64_t kMaxChunks = 0x7fffffffll / (kChunk / kAdamPart);      // (workgroups of a launch are counted in 31 bits)
+// A launch counts its threads in 32 bits: fewer than 2^24 workgroups.  (The norm's are few; its chunks are counted in 31 bits.)
+constexpr int64_t kMaxGrid = (1ll << 32) / kThreads - 1;
+int64_t max_chunks(int form) {
+    return form == kFormNorm ? 1ll << 30 : kMaxGrid / (kChunk / (form == kFormClip ? kClipPartWide : kAdamPart));
+}
 int64_t padded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // a range of memory that the call writes (or only reads), for the overlap check
@@ -599,7 +603,7 @@ int build(const char* what, const Item* items, int64_t count, int form, int grou
             s.first = (int)chunks;
             list.push_back(s);
             chunks += chunks_of(s, chunk);
-            NIW_REQUIRE(chunks <= kMaxChunks, "%s: more than %lld chunks of %d elements", what, (long long)kMaxChunks, chunk);
+            NIW_REQUIRE(chunks <= max_chunks(form), "%s: more than %lld chunks of %d elements", what, (long long)max_chunks(form), chunk);
         }
     }
     slots = (int)list.size();

@@ -352,10 +352,13 @@ def _types(tensors):
     return [DTYPES[t.dtype] for t in tensors]
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """makes the list's GPU current for a launch (its stream and allocations are that GPU's)"""
     if device is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(device)
 
 
@@ -371,7 +374,7 @@ class _Table:
         self._c = _lib.Table()
         if getattr(lib, name)(ctypes.c_void_p(rows.ctypes.data), len(rows), *how, image, ctypes.byref(self._c)):
             raise _lib.NiwError(lib.niw_last_error_string().decode())
-        self._stream, self._image = None, None
+        self._streams, self._image = set(), None
         if self._c.bytes:
             if kept and torch.cuda.is_current_stream_capturing():
                 raise _lib.NiwError(f"{type(self).__name__}: build the table before the capture begins")
@@ -380,7 +383,7 @@ class _Table:
                 self._c.image = self._image.data_ptr()
                 stream = torch.cuda.current_stream()
                 _lib.call("niw_table_store", image, self._c.bytes, _p(self._image), ctypes.c_void_p(stream.cuda_stream))
-                self._stream = stream.cuda_stream
+                self._streams.add(stream.cuda_stream)
                 if kept:
                     stream.synchronize()
 
@@ -388,8 +391,9 @@ class _Table:
         """the current stream of the list's GPU (its handle alone: a torch.cuda.Stream object costs 2.5 us of a 14 us call), which the image is
         kept alive for"""
         handle = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
-        if handle != self._stream and self._image is not None:
+        if handle not in self._streams and self._image is not None:
             self._image.record_stream(torch.cuda.current_stream())
+            self._streams.add(handle)
         return handle
 
 
@@ -459,7 +463,7 @@ def grad_total(grads, norm_type=2.0):
         total = torch.empty(1, device=table.device or "cuda", dtype=torch.float64)
         ws = _norm_workspace(total.device)
         with timed("grad_norm", table.numel):
-            _lib.call("niw_grad_norm", ctypes.byref(table._c), kind, _p(ws), _p(total), None, table._use())
+            _lib.call("niw_grad_norm", ctypes.byref(table._c), kind, ws.data_ptr(), total.data_ptr(), None, table._use())
     return total
 
 
@@ -471,18 +475,19 @@ def grad_norm(grads, norm_type=2.0):
         norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
         ws = _norm_workspace(norm.device)
         with timed("grad_norm", table.numel):
-            _lib.call("niw_grad_norm", ctypes.byref(table._c), kind, _p(ws), None, _p(norm), table._use())
+            _lib.call("niw_grad_norm", ctypes.byref(table._c), kind, ws.data_ptr(), None, norm.data_ptr(), table._use())
     return norm
 
 
 def _total(total, device):
+    """-> (total, the device to run on): that of the tensors, of the total where there are none"""
     if total is None:
-        return None
+        return None, device
     if not (isinstance(total, torch.Tensor) and total.is_cuda and total.dtype == torch.float64 and total.numel() == 1):
         raise _lib.NiwError("total: the [1] float64 tensor of grad_total")
     if device is not None and total.device != device:
         raise _lib.NiwError(f"total is on {total.device}, the tensors on {device}")
-    return total
+    return total, total.device
 
 
 def _max_norm(max_norm):
@@ -500,9 +505,9 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None, total=None):
     table, kind, max_norm = _table(grads, out), _norm_kind(norm_type), _max_norm(max_norm)
     if table._unclippable:
         raise _lib.NiwError(table._unclippable)
-    total = _total(total, table.device)
-    with _on(table.device):
-        norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
+    total, device = _total(total, table.device)
+    with _on(device):
+        norm = torch.empty((), device=device or "cuda", dtype=torch.float32)
         ws = _norm_workspace(norm.device) if total is None else None
         with timed("clip_grads", table.numel):
             _lib.call("niw_grad_clip", ctypes.byref(table._c), kind, max_norm, _p(total), _p(ws), _p(norm), table._use())
@@ -587,7 +592,7 @@ def adam_step_tensors(tensors, lr, step, weight_decay=0.0, beta1=0.9, beta2=0.99
     for t, shape, name in ((hyper_dev, 2 * n, "hyper_dev"), (decay_dev, n, "decay_dev")):
         if t is not None and (_f32(t, name) is not t or t.numel() != shape or t.device != (table.device or t.device)):
             raise _lib.NiwError(f"{name}: a contiguous float32 tensor of {shape} values on the parameters' device")
-    hyper = (_lib.AdamHyper * n)(*[_lib.AdamHyper(lr=a, weight_decay=b, step=c) for a, b, c in zip(lr, decay, step)])
+    hyper = (_lib.AdamHyper * n)(*zip(lr, decay, step))
     if max_norm is None:
         if skip_nonfinite or total is not None:
             raise _lib.NiwError("adam_step_tensors: skip_nonfinite and total go with max_norm (math.inf clips nothing)")
@@ -595,9 +600,9 @@ def adam_step_tensors(tensors, lr, step, weight_decay=0.0, beta1=0.9, beta2=0.99
             _lib.call("niw_adam_step_tensors", ctypes.byref(table._c), hyper, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev), None,
                       table._use())
         return None
-    total, kind, max_norm = _total(total, table.device), _norm_kind(norm_type), _max_norm(max_norm)
-    with _on(table.device):
-        norm = torch.empty((), device=table.device or "cuda", dtype=torch.float32)
+    (total, device), kind, max_norm = _total(total, table.device), _norm_kind(norm_type), _max_norm(max_norm)
+    with _on(device):
+        norm = torch.empty((), device=device or "cuda", dtype=torch.float32)
         ws = _norm_workspace(norm.device) if total is None else None
         clip = _lib.AdamClip(max_norm=max_norm, kind=kind, skip_nonfinite=1 if skip_nonfinite else 0, total=None if total is None else total.data_ptr(),
                              workspace=None if ws is None else ws.data_ptr(), norm=norm.data_ptr())

@@ -223,6 +223,7 @@ def test_total_of_several_shares():
         assert abs(float(norm) - want) <= H * want * (1 + 1e-6)
     for x, y in zip(a + b, before):
         check_clipped(x, y, coefficient(want, 3.0))
+    assert abs(float(ops.clip_grads([], 3.0, total=total)) - want) <= H * want * (1 + 1e-6)          # a rank whose share is empty
     with pytest.raises(_lib.NiwError, match="grad_total"):
         ops.clip_grads(a, 1.0, total=torch.zeros(1, device=DEV))
 

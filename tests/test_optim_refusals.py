@@ -76,7 +76,18 @@ def test_c_table_counts_what_it_holds():
     rc, t = grad_table([(1 << 40, 1 << 40, 1 << 33, 0, 0)], 1)
     assert rc == 0 and t.chunks == (1 << 33) // t.chunk
     assert grad_table([], 1)[1].slots == 0
+
+
+def test_c_lists_whose_launch_could_not_be_counted_are_refused():
+    """a launch has less than 2^32 threads: 2^24 workgroups of 256, one per 1024 elements of an update and per 2048 (or 4096) of a clip"""
+    far = 1 << 60
     assert grad_table([(1024, 2048, 1 << 44, 0, 0)] * 3, 0)[0] == -1 and "chunks" in err()
+    assert grad_table([(1024, 1024, (1 << 35) - (1 << 15), 0, 0)], 1)[0] == 0
+    assert grad_table([(1024, 1024, 1 << 35, 0, 0)], 1)[0] == -1 and "chunks" in err()
+    assert grad_table([(1024, 1024, 1 << 35, 0, 0)], 0)[0] == 0
+    big = dict(param=far, grad=2 * far, exp_avg=3 * far, exp_avg_sq=4 * far)
+    assert adam_table(n=(1 << 34) - (1 << 14), **big)[0] == 0
+    assert adam_table(n=1 << 34, **big)[0] == -1 and "chunks" in err()
 
 
 @pytest.mark.parametrize("lengths", [[1], [4096], [4097], [530052, 530052, 165900, 2304], [5] * 3000, [100000] * 100, [1 << 20] * 5, [1 << 20] * 16, [3, 7]])
