@@ -5,6 +5,7 @@ streams and the autograd tape here; every number is produced by libniw_hip.so.
 import ctypes
 import contextlib
 import math
+import operator
 
 import numpy as np
 import torch
@@ -310,11 +311,22 @@ def _check_dense(t, name):
         run *= n
 
 
-def _check_all(tensors, name):
-    """_check_dense of a list whose tensors are nearly always plain: a quick look at all of them first"""
-    if not all(isinstance(t, torch.Tensor) and t.dtype in DTYPES and t.layout is torch.strided and t.is_contiguous() and not t.is_neg() for t in tensors):
+_T, _DTYPE, _LAYOUT = torch.Tensor, operator.attrgetter("dtype"), operator.attrgetter("layout")
+
+
+def _gather(tensors, name):
+    """-> (addresses, lengths, types, whether all are contiguous) of a list of dense tensors.  Nearly always all are plain, and a list has
+    hundreds: each property is asked for in one sweep (a microsecond per tensor), a tensor is looked at closely only where a sweep finds one."""
+    try:
+        plain = all(map(_T.is_contiguous, tensors)) and not any(map(_T.is_neg, tensors)) and set(map(_LAYOUT, tensors)) <= {torch.strided}
+        types = [DTYPES[d] for d in map(_DTYPE, tensors)]
+    except (TypeError, KeyError, RuntimeError):
+        plain, types = False, None
+    if not plain:
         for i, t in enumerate(tensors):
             _check_dense(t, f"{name} {i}")
+        types = [DTYPES[t.dtype] for t in tensors]
+    return list(map(_T.data_ptr, tensors)), list(map(_T.numel, tensors)), types, plain
 
 
 def _check_pairs(first, second, name):
@@ -327,29 +339,21 @@ def _check_pairs(first, second, name):
 
 def _check_device(tensors, name):
     """the one GPU all of them are on (None: an empty list)"""
-    if not tensors:
-        return None
-    device = tensors[0].device
-    if any(t.get_device() != device.index if device.type == "cuda" else True for t in tensors):
-        devices = {t.device for t in tensors}
-        if len(devices) > 1:
-            raise _lib.NiwError(f"{name}: tensors on several devices ({', '.join(sorted(map(str, devices)))})")
-        raise _lib.NiwError(f"{name}: expected CUDA/HIP tensors, got {device}")
-    return device
+    indices = set(map(_T.get_device, tensors))
+    if len(indices) == 1 and tensors[0].is_cuda:
+        return tensors[0].device
+    devices = {t.device for t in tensors}
+    if len(devices) > 1:
+        raise _lib.NiwError(f"{name}: tensors on several devices ({', '.join(sorted(map(str, devices)))})")
+    if devices:
+        raise _lib.NiwError(f"{name}: expected CUDA/HIP tensors, got {devices.pop()}")
+    return None
 
 
 # rows of niw_grad_tensor / niw_adam_tensor (include/niw.h); a list's are filled column by column
 _GRAD_ROW = np.dtype([("grad", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("out_dtype", "<i4")])
 _ADAM_ROW = np.dtype([("param", "<u8"), ("grad", "<u8"), ("exp_avg", "<u8"), ("exp_avg_sq", "<u8"), ("master", "<u8"), ("n", "<i8"), ("param_dtype", "<i4"),
                       ("grad_dtype", "<i4"), ("group", "<i4"), ("reserved", "<i4")])
-
-
-def _addresses(tensors):
-    return [t.data_ptr() for t in tensors]
-
-
-def _types(tensors):
-    return [DTYPES[t.dtype] for t in tensors]
 
 
 _HERE = contextlib.nullcontext()
@@ -418,18 +422,18 @@ class TensorTable(_Table):
         given = sum(o is not None for o in out)
         if given not in (0, len(out)):
             raise _lib.NiwError("TensorTable: an output for some tensors only")
-        _check_all(tensors, "tensor")
-        if given:
-            _check_all(out, "output")
-            _check_pairs(tensors, out, "output")
-        else:
-            out = tensors
-        every = tensors + out if given else tensors
-        self.device = _check_device(every, "TensorTable")
         rows = np.zeros(len(tensors), _GRAD_ROW)
-        rows["grad"], rows["out"], rows["n"] = _addresses(tensors), _addresses(out), [t.numel() for t in tensors]
-        rows["dtype"], rows["out_dtype"] = _types(tensors), _types(out)
-        self.numel = int(rows["n"].sum())
+        rows["grad"], lengths, rows["dtype"], plain = _gather(tensors, "tensor")
+        rows["n"], every = lengths, tensors
+        if given:
+            rows["out"], out_lengths, rows["out_dtype"], out_plain = _gather(out, "output")
+            if lengths != out_lengths or not (plain and out_plain):
+                _check_pairs(tensors, out, "output")
+            every = tensors + out
+        else:
+            rows["out"], rows["out_dtype"] = rows["grad"], rows["dtype"]
+        self.device = _check_device(every, "TensorTable")
+        self.numel = sum(lengths)
         kept = TABLE_KEPT if _kept else 0
         self._unclippable = None
         try:
@@ -545,28 +549,29 @@ class AdamTable(_Table):
             master += [lists["master"][i] for i in keep]
             group += [k] * len(keep)
         masters = [t for t in master if t is not None]
-        for key in names:
-            _check_all(cols[key], key)
-        _check_all(masters, "master")
-        for key, t in [(key, t) for key in names[2:] for t in cols[key]] + [("master", t) for t in masters]:
-            if t.dtype != torch.float32:
-                raise _lib.NiwError(f"AdamTable: {key}: expected float32, got {t.dtype}")
-        for p, w in zip(cols["params"], master):
-            if (p.dtype == torch.float32) != (w is None):
-                raise _lib.NiwError("AdamTable: a half-precision parameter needs a float32 master copy (updates below half a step of its type would be "
-                                    "lost), a float32 parameter has none")
+        rows = np.zeros(len(group), _ADAM_ROW)
+        rows["group"], rows["master"] = group, 0
+        plain, lengths, types = {}, {}, {}
+        for field, key in zip(("param", "grad", "exp_avg", "exp_avg_sq"), names):
+            rows[field], lengths[key], types[key], plain[key] = _gather(cols[key], key)
+        own, _, types["master"], plain["master"] = _gather(masters, "master")
+        for key in names[2:] + ("master",):
+            if any(types[key]):
+                raise _lib.NiwError(f"AdamTable: {key}: expected float32, got {next(t.dtype for t in cols.get(key, masters) if t.dtype != torch.float32)}")
+        with_master = [w is not None for w in master]
+        if [bool(t) for t in types["params"]] != with_master:
+            raise _lib.NiwError("AdamTable: a half-precision parameter needs a float32 master copy (updates below half a step of its type would be "
+                                "lost), a float32 parameter has none")
         for key in names[1:]:
-            _check_pairs(cols["params"], cols[key], key)
+            if lengths[key] != lengths["params"] or not (plain[key] and plain["params"]):
+                _check_pairs(cols["params"], cols[key], key)
         _check_pairs([p for p, w in zip(cols["params"], master) if w is not None], masters, "master")
+        rows["master"][np.array(with_master, dtype=bool)] = own
+        rows["n"], rows["param_dtype"], rows["grad_dtype"] = lengths["params"], types["params"], types["grads"]
         tensors = [t for key in names for t in cols[key]] + masters
         self.device = _check_device(tensors, "AdamTable")
         self.n_groups = len(groups)
-        rows = np.zeros(len(group), _ADAM_ROW)
-        for field, key in zip(("param", "grad", "exp_avg", "exp_avg_sq"), names):
-            rows[field] = _addresses(cols[key])
-        rows["master"], rows["n"], rows["group"] = [0 if w is None else w.data_ptr() for w in master], [p.numel() for p in cols["params"]], group
-        rows["param_dtype"], rows["grad_dtype"] = _types(cols["params"]), _types(cols["grads"])
-        self.numel = int(rows["n"].sum())
+        self.numel = sum(lengths["params"])
         self._build("niw_adam_table", rows, (self.n_groups, TABLE_KEPT if _kept else 0), tensors, _kept)
 
 
