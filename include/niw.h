@@ -404,8 +404,8 @@ typedef struct niw_grad_tensor {
 typedef struct niw_table {      /* HOST; everything but `image` is filled by niw_grad_table / niw_adam_table and opaque */
     const void* image;          /* device, 16-byte aligned: set by the caller to where the image was stored */
     int64_t bytes;              /* of the image */
-    int32_t form, slots, chunks, chunk, groups, wide;
-    int64_t read, moved;
+    int32_t form, slots, chunks, chunk, groups, wide, parts, reserved;
+    int64_t read, touched;
 } niw_table;
 
 /* NIW_TABLE_CLIP: a table for niw_grad_clip too (without: for niw_grad_norm alone).  NIW_TABLE_KEPT: a table for many calls, whose image may

@@ -38,7 +38,7 @@ class GradTensor(ctypes.Structure):
 class Table(ctypes.Structure):
     """niw_table of include/niw.h"""
     _fields_ = [("image", _vp), ("bytes", _i64), ("form", _i32), ("slots", _i32), ("chunks", _i32), ("chunk", _i32), ("groups", _i32), ("wide", _i32),
-                ("read", _i64), ("moved", _i64)]
+                ("parts", _i32), ("reserved", _i32), ("read", _i64), ("touched", _i64)]
 
 
 class AdamTensor(ctypes.Structure):

@@ -34,7 +34,6 @@ constexpr double kClipEps = 1e-6;
 constexpr int kChunk = 16384, kSmallChunk = 4096;
 constexpr long long kSmallList = 1024ll * kChunk;
 constexpr int kMaxPieces = 2048;               // (of a kept small list: see build)
-constexpr int kRound = 2048;
 // The norm runs on at most kNormBlocks workgroups, four per compute unit, that walk the list with its whole width: 1 GB and up read at
 // 7.0 TB/s with 1024, 6.7 with 2048 or 4096, 6.8 with 512 (which costs half-precision lists a quarter: their conversions want more waves).
 constexpr int kNormBlocks = 1024;
@@ -52,8 +51,9 @@ constexpr int kAdamStretch = 64, kClipStretchWide = 32;
 // The workgroups of a clip or an update join the norm's partial sums themselves as long as they are few (kFoldGrid): saves a launch,
 // 3 us of the trainer's 18; with 120,000 workgroups one more launch is cheaper (2 GB in place: 963 us against 973).
 constexpr int kFoldGrid = 4096;
-// Lists that move more than the 256 MB of memory-side cache hold go past the caches (non-temporal); a norm still leaves the last
-// kCache bytes of gradients in it, which the clip or update behind it reads first: it walks the list backwards.
+// Lists that touch more than the memory-side cache can keep (256 MB, of which other work has a part) go past the caches, non-temporal: Adam
+// of 335 M bf16 parameters 1.91 -> 1.74 ms, but of 8 M fp32 ones (128 MB) 35 -> 45 us.  A norm still leaves the last kCache bytes of
+// gradients there, which the clip or update behind it reads first: it walks the list backwards.
 constexpr int64_t kCache = 192ll << 20;
 
 // ------------------------------------------------------------------------------------------------ the image of a list
@@ -82,7 +82,7 @@ static_assert(sizeof(GradSlot) == 32 && sizeof(AdamSlot) == 64, "slots are read 
 template <class Slot>
 struct List {
     const Slot* slots;
-    int count, chunks, chunk;
+    int count, chunks, chunk, parts;
     // the slot of chunk c: its own number in a list whose tensors have a chunk each
     __device__ __forceinline__ int slot_of(int c) const;
 };
@@ -154,14 +154,6 @@ __device__ __forceinline__ long long odd_element(int head, long long begin, long
     if (tid < head) return begin + tid;
     return tid >= kThreads / 2 && tid < kThreads / 2 + tail ? end - tail + (tid - kThreads / 2) : -1;
 }
-// Parts of `part` elements that a chunk is cut into; in small lists no more than one round of workgroups, eight per compute unit (Adam of
-// 600 vectors 16.7 -> 14.3 us).
-template <class Slot>
-__host__ __device__ inline int parts_of(const List<Slot>& list, int part) {
-    int n = list.chunk > part ? list.chunk / part : 1;
-    while (list.chunk == kSmallChunk && n > 1 && list.chunks * n > kRound) n /= 2;
-    return n;
-}
 // the part of this workgroup (one workgroup per part), from the list's end backwards; any = false: nothing is left for it
 template <class Slot>
 struct Part {
@@ -170,14 +162,14 @@ struct Part {
     int head;
     bool any;
 };
-template <int PART, int STRETCH, class Slot>
+template <int STRETCH, class Slot>
 __device__ __forceinline__ Part<Slot> part_of(const List<Slot>& list) {
     // workgroups go to the eight dies in turn: of every 8 x STRETCH parts each die takes STRETCH that follow each other
     constexpr unsigned kDies = 8, kGroup = kDies * STRETCH;
     unsigned at_grid = blockIdx.x;
     const unsigned group = at_grid / kGroup * kGroup;
     if (STRETCH > 1 && group + kGroup <= gridDim.x) at_grid = group + at_grid % kDies * STRETCH + (at_grid - group) / kDies;
-    const int split = parts_of(list, PART), b = (int)at_grid / split, part = split - 1 - (int)at_grid % split;
+    const int split = list.parts, b = (int)at_grid / split, part = split - 1 - (int)at_grid % split;
     const int c = list.chunks - 1 - b;
     Part<Slot> p{};
     if (c < 0) return p;
@@ -383,7 +375,7 @@ __device__ __forceinline__ Factor clip_factor(const Clip& clip) {
 template <int KIND, bool NT, int PART>
 __global__ __launch_bounds__(kThreads) void clip_kernel(List<GradSlot> list, Clip clip) {
     const float c = clip_factor<KIND>(clip).c;
-    const auto part = part_of<PART, PART == kClipPartWide ? kClipStretchWide : 1>(list);
+    const auto part = part_of<PART == kClipPartWide ? kClipStretchWide : 1>(list);
     const GradSlot& s = part.s;
     if (!part.any || (c == 1.f && s.o == s.g)) return;
     with_dtype(s.types & 255, [&](auto gt) {
@@ -414,10 +406,11 @@ struct AdamArgs {
 
 // The update, one part of 1024 elements per workgroup: four elements of every stream per thread, 28 to 30 bytes each, and nothing reused.
 // 335 M bf16 parameters with master copies 1489 us, 101 M fp32 with fp16 gradients in unaligned tensors 408 us.
-template <int KIND, bool NT>
+// DECAY: some group of the call decays (without, an infinite parameter is not multiplied by 0 either).
+template <int KIND, bool NT, bool DECAY>
 __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> list, AdamArgs a, Clip clip) {
     const Factor factor = clip_factor<KIND>(clip);
-    const auto part = part_of<kAdamPart, kAdamStretch>(list);
+    const auto part = part_of<kAdamStretch>(list);
     if (!part.any || factor.skip) return;
     const AdamSlot& s = part.s;
     const int k = __builtin_amdgcn_readfirstlane(s.types >> 16), tid = threadIdx.x;
@@ -427,14 +420,8 @@ __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> l
     with_dtype(s.types & 255, [&](auto gt) {
         with_dtype((s.types >> 8) & 255, [&](auto pt) {
             constexpr int G = decltype(gt)::value, P = decltype(pt)::value;
-            struct Four {
-                f32x4 p, m, v, g;
-            };
-            auto read = [&](long long i) {
-                return Four{load4<NT, NIW_F32>(w, i), load4<NT, NIW_F32>(s.m, i), load4<NT, NIW_F32>(s.v, i), load4<NT, G>(s.g, i)};
-            };
             auto update = [&](float& p, float g, float& m, float& v) {
-                p = fmaf(-decay, p, p);
+                if constexpr (DECAY) p = fmaf(-decay, p, p);
                 niw::adam_update(p, niw::mul_rn(factor.c, g), m, v, a.w1, a.b2, a.w2, a.eps, step_size, bc2_sqrt);
             };
             const long long odd = odd_element<4>(part.head, part.begin, part.end);
@@ -445,17 +432,18 @@ __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> l
                 if constexpr (P != NIW_F32) store1<P>(s.p, odd, p);
             }
             for (long long i = part.begin + part.head + tid * 4; i + 4 <= part.end; i += kThreads * 4) {
-                Four x = read(i);
+                f32x4 p = load4<NT, NIW_F32>(w, i), m = load4<NT, NIW_F32>(s.m, i), v = load4<NT, NIW_F32>(s.v, i);
+                const f32x4 g = load4<NT, G>(s.g, i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float pj = x.p[j], mj = x.m[j], vj = x.v[j];
-                    update(pj, x.g[j], mj, vj);
-                    x.p[j] = pj; x.m[j] = mj; x.v[j] = vj;
+                    float pj = p[j], mj = m[j], vj = v[j];
+                    update(pj, g[j], mj, vj);
+                    p[j] = pj; m[j] = mj; v[j] = vj;
                 }
-                store4<NT, NIW_F32>(w, i, x.p);
-                store4<NT, NIW_F32>(s.m, i, x.m);
-                store4<NT, NIW_F32>(s.v, i, x.v);
-                if constexpr (P != NIW_F32) store4<NT, P>(s.p, i, x.p);
+                store4<NT, NIW_F32>(w, i, p);
+                store4<NT, NIW_F32>(s.m, i, m);
+                store4<NT, NIW_F32>(s.v, i, v);
+                if constexpr (P != NIW_F32) store4<NT, P>(s.p, i, p);
             }
         });
     });
@@ -557,13 +545,15 @@ void fill(AdamSlot& s, const niw_adam_tensor& t) {
     s.types = t.grad_dtype | t.param_dtype << 8 | t.group << 16;
 }
 
-// bytes of gradients, and bytes that a clip or an update of the tensor moves
-void read_written(const niw_grad_tensor& t, int64_t& read, int64_t& moved) {
-    read += t.n * size_of(t.dtype); moved += t.n * (size_of(t.dtype) + size_of(t.out_dtype));
+// bytes of gradients, and bytes that a clip or an update of the tensor touches
+void count_bytes(const niw_grad_tensor& t, int64_t& read, int64_t& touched) {
+    read += t.n * size_of(t.dtype); touched += t.n * (size_of(t.dtype) + (t.out == t.grad ? 0 : size_of(t.out_dtype)));
 }
-void read_written(const niw_adam_tensor& t, int64_t& read, int64_t& moved) {
-    read += t.n * size_of(t.grad_dtype); moved += t.n * (24 + size_of(t.grad_dtype) + (t.master ? 2 : 0));
+void count_bytes(const niw_adam_tensor& t, int64_t& read, int64_t& touched) {
+    read += t.n * size_of(t.grad_dtype); touched += t.n * (12 + size_of(t.grad_dtype) + (t.master ? 2 : 0));
 }
+int bytes_per_element(const niw_grad_tensor& t) { return size_of(t.dtype) + size_of(t.out_dtype); }
+int bytes_per_element(const niw_adam_tensor&) { return 0; }
 
 // the elements [at, at + n) of a slot
 void advance(GradSlot& s, long long at, long long n) {
@@ -581,13 +571,14 @@ void advance(AdamSlot& s, long long at, long long n) {
 
 template <class Slot, class Item>
 int build(const char* what, const Item* items, int64_t count, int form, int groups, bool kept, void* image, niw_table* table) {
-    long long total = 0, pieces = 0;
+    long long total = 0, pieces = 0, wide = 0;
     int slots = 0;
     *table = niw_table{};
     for (int64_t i = 0; i < count; ++i) {
         total += items[i].n; slots += items[i].n > 0;
         pieces += items[i].n / (kSmallChunk - kLine) + 1;
-        read_written(items[i], table->read, table->moved);
+        count_bytes(items[i], table->read, table->touched);
+        wide += items[i].n * bytes_per_element(items[i]);
     }
     const int chunk = total < kSmallList ? kSmallChunk : kChunk;
     // small lists that are kept: a slot per chunk, so that no workgroup has to search
@@ -616,7 +607,11 @@ int build(const char* what, const Item* items, int64_t count, int form, int grou
     }
     slots = (int)list.size();
     table->form = form; table->slots = slots; table->chunks = (int)chunks; table->chunk = chunk; table->groups = groups;
-    table->wide = table->moved >= 8 * total;
+    table->wide = wide >= 8 * total;
+    // as many parts as a chunk has on the average
+    const int part = form == kFormAdam ? kAdamPart : table->wide ? kClipPartWide : kClipPart;
+    table->parts = 1;
+    while (table->parts * part < chunk && table->parts * part * chunks < total) table->parts *= 2;
     table->bytes = padded((int64_t)slots * (sizeof(Slot) + sizeof(int)));
     if (!slots) return NIW_OK;
     memset(image, 0, table->bytes);
@@ -628,7 +623,7 @@ int build(const char* what, const Item* items, int64_t count, int form, int grou
 
 template <class Slot>
 List<Slot> list_of(const niw_table& t) {
-    return List<Slot>{static_cast<const Slot*>(t.image), t.slots, t.chunks, t.chunk};
+    return List<Slot>{static_cast<const Slot*>(t.image), t.slots, t.chunks, t.chunk, t.parts};
 }
 int check_table(const char* what, const niw_table* t, bool form_fits) {
     NIW_REQUIRE(t, "%s: null pointer", what);
@@ -653,10 +648,15 @@ void launch_finish(int kind, const double* partial, int n, double* total, float*
     if (kind == NIW_NORM_2) finish_kernel<NIW_NORM_2><<<1, kThreads, 0, st>>>(partial, n, total, norm);
     else finish_kernel<NIW_NORM_MAX><<<1, kThreads, 0, st>>>(partial, n, total, norm);
 }
+template <class F>
+void with_bool(bool value, F f) {
+    if (value) f(std::true_type{});
+    else f(std::false_type{});
+}
 // one workgroup per part (one for an empty list, whose norm is still written)
 template <class Slot>
-int64_t grid_of(const List<Slot>& list, int part) {
-    return list.chunks < 1 ? 1 : (int64_t)list.chunks * parts_of(list, part);
+int64_t grid_of(const List<Slot>& list) {
+    return list.chunks < 1 ? 1 : (int64_t)list.chunks * list.parts;
 }
 // the norm's launches in front of a kernel of `grid` workgroups that clips by it
 template <class Slot>
@@ -732,22 +732,16 @@ extern "C" int niw_grad_clip(const niw_table* table, int kind, double max_norm, 
     hipStream_t st = (hipStream_t)stream;
     const auto list = list_of<GradSlot>(*table);
     Clip clip{nullptr, norm_out, max_norm, 1, 0};
-    const bool nt = table->moved > kCache, wide = table->wide != 0;
-    const int64_t grid = grid_of(list, wide ? kClipPartWide : kClipPart);
+    const int64_t grid = grid_of(list);
     prepare_clip(clip, list, *table, grid, kind, total, workspace, st);
-    auto launch = [&](auto nk, auto past, auto part) {
-        clip_kernel<decltype(nk)::value, decltype(past)::value, decltype(part)::value><<<(unsigned)grid, kThreads, 0, st>>>(list, clip);
-    };
-    auto with_part = [&](auto nk, auto past) {
-        if (wide) launch(nk, past, std::integral_constant<int, kClipPartWide>{});
-        else launch(nk, past, std::integral_constant<int, kClipPart>{});
-    };
-    auto with_nt = [&](auto nk) {
-        if (nt) with_part(nk, std::true_type{});
-        else with_part(nk, std::false_type{});
-    };
-    if (kind == NIW_NORM_2) with_nt(std::integral_constant<int, NIW_NORM_2>{});
-    else with_nt(std::integral_constant<int, NIW_NORM_MAX>{});
+    with_bool(table->touched > kCache, [&](auto nt) {
+        with_bool(table->wide != 0, [&](auto wide) {
+            constexpr bool N = decltype(nt)::value;
+            constexpr int P = decltype(wide)::value ? kClipPartWide : kClipPart;
+            if (kind == NIW_NORM_2) clip_kernel<NIW_NORM_2, N, P><<<(unsigned)grid, kThreads, 0, st>>>(list, clip);
+            else clip_kernel<NIW_NORM_MAX, N, P><<<(unsigned)grid, kThreads, 0, st>>>(list, clip);
+        });
+    });
     NIW_LAUNCH_CHECK("niw_grad_clip");
     return NIW_OK;
 }
@@ -775,7 +769,7 @@ extern "C" int niw_adam_step_tensors(const niw_table* table, const niw_adam_hype
     a.hyper_dev = hyper_dev; a.decay_dev = decay_dev;
     hipStream_t st = (hipStream_t)stream;
     const auto list = list_of<AdamSlot>(*table);
-    const int64_t grid = grid_of(list, kAdamPart);
+    const int64_t grid = grid_of(list);
     Clip c{};
     if (clip) {
         NIW_REQUIRE(clip->kind == NIW_NORM_2 || clip->kind == NIW_NORM_MAX, "niw_adam_step_tensors: unknown kind %d", clip->kind);
@@ -784,10 +778,15 @@ extern "C" int niw_adam_step_tensors(const niw_table* table, const niw_adam_hype
         c.norm_out = clip->norm; c.max_norm = clip->max_norm; c.skip_nonfinite = clip->skip_nonfinite;
         prepare_clip(c, list, *table, grid, clip->kind, clip->total, clip->workspace, st);
     }
-    const bool nt = table->moved > kCache;
-    auto* const kernel = !clip || clip->kind == NIW_NORM_2 ? (nt ? adam_tensors_kernel<NIW_NORM_2, true> : adam_tensors_kernel<NIW_NORM_2, false>)
-                                                           : (nt ? adam_tensors_kernel<NIW_NORM_MAX, true> : adam_tensors_kernel<NIW_NORM_MAX, false>);
-    kernel<<<(unsigned)grid, kThreads, 0, st>>>(list, a, c);
+    bool decays = decay_dev != nullptr;
+    for (int k = 0; k < table->groups; ++k) decays |= a.decay[k] != 0.f;
+    with_bool(table->touched > kCache, [&](auto nt) {
+        with_bool(decays, [&](auto decay) {
+            constexpr bool N = decltype(nt)::value, D = decltype(decay)::value;
+            if (!clip || clip->kind == NIW_NORM_2) adam_tensors_kernel<NIW_NORM_2, N, D><<<(unsigned)grid, kThreads, 0, st>>>(list, a, c);
+            else adam_tensors_kernel<NIW_NORM_MAX, N, D><<<(unsigned)grid, kThreads, 0, st>>>(list, a, c);
+        });
+    });
     NIW_LAUNCH_CHECK("niw_adam_step_tensors");
     return NIW_OK;
 }

@@ -303,6 +303,8 @@ def test_adam_groups_have_their_own_values():
 def test_adam_without_a_clip_that_bites_has_the_bits_of_adam_step_multi():
     lengths = [530052, 165900, 2304, 1]
     a = adam_state(lengths, F32, F32)
+    for x, value in ((a["params"][0], math.inf), (a["params"][1], -math.inf), (a["exp_avg"][0], 0.0), (a["exp_avg_sq"][0], 0.0)):
+        x[5::1000] = value
     b, c = copy_state(a), copy_state(a)
     rows = lambda s: [(s["params"][i], s["grads"][i], s["exp_avg"][i], s["exp_avg_sq"][i], 1e-3, 5) for i in range(len(lengths))]
     for _ in range(3):
@@ -310,7 +312,9 @@ def test_adam_without_a_clip_that_bites_has_the_bits_of_adam_step_multi():
         ops.adam_step_tensors([b], lr=1e-3, step=5)
         ops.adam_step_tensors([c], lr=1e-3, step=5, max_norm=math.inf)
     for k in ("params", "exp_avg", "exp_avg_sq"):
-        assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(a[k], b[k], c[k]))
+        bits = lambda s: [x.view(torch.int32) for x in s[k]]
+        assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(bits(a), bits(b), bits(c)))
+    assert math.isinf(float(a["params"][0][5])) and math.isinf(float(c["params"][1][5]))
 
 
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
@@ -473,6 +477,30 @@ def test_captured_and_replayed():
         assert float(norm1) == float(clipped1) == float(want) and float(norm2) == float(used)
         for k in ("params", "master", "grads", "exp_avg", "exp_avg_sq"):
             assert all(torch.equal(x, y) for x, y in zip(s[k], e[k])), (step, k)
+
+
+def test_two_graphs_of_one_table_at_the_same_time():
+    """each graph has a workspace of its own: replayed on two streams at once, against lists that change in between"""
+    g = [rand(n, BF16, seed=n) for n in (3_000_001, 5, 70001)]
+    table = ops.TensorTable(g)
+    ops.grad_norm(table)
+    torch.cuda.synchronize()
+    graphs, results, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for kind in (2.0, math.inf):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append([ops.grad_norm(table, norm_type=kind) for _ in range(8)])
+    for trial in range(5):
+        for i, x in enumerate(g):
+            x.copy_(rand(x.numel(), BF16, seed=trial * 10 + i))
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for norms, kind in zip(results, (2.0, math.inf)):
+            for n in norms:
+                check_norm(n, g, kind)
 
 
 def test_a_table_is_built_in_front_of_a_capture_a_list_may_be_gathered_inside():
