@@ -291,50 +291,60 @@ def _norm_kind(norm_type):
     return kind
 
 
-def _layout(t):
-    """the dimensions that say which element lies where: (size, stride) without those of size 1, outermost first"""
-    return tuple((n, s) for n, s in zip(t.shape, t.stride()) if n != 1)
+MAX_RUNS = 1 << 18          # gap-free stretches that one tensor of a list may consist of (each is an entry of its own)
 
 
-def _check_dense(t, name):
-    """every element of the tensor in one gap-free run of memory, in whatever order: an elementwise pass may then walk that run"""
+def _check_tensor(t, name):
     if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES:
         raise _lib.NiwError(f"{name}: expected a float32, bfloat16 or float16 tensor, got {type(t).__name__} {getattr(t, 'dtype', '')}")
     if t.layout != torch.strided or t.is_neg():
         raise _lib.NiwError(f"{name}: expected a strided tensor that holds its own values, got {t.layout}{', a negated view' if t.is_neg() else ''}")
-    if t.is_contiguous() or t.numel() == 0:
-        return
-    run = 1
-    for n, s in sorted(_layout(t), key=lambda d: d[1]):
-        if s != run:
-            raise _lib.NiwError(f"{name}: shape {tuple(t.shape)} with strides {t.stride()} has gaps or shares elements; pass a dense tensor")
-        run *= n
 
 
 _T, _DTYPE, _LAYOUT = torch.Tensor, operator.attrgetter("dtype"), operator.attrgetter("layout")
 
 
 def _gather(tensors, name):
-    """-> (addresses, lengths, types, whether all are contiguous) of a list of dense tensors.  Nearly always all are plain, and a list has
-    hundreds: each property is asked for in one sweep (a microsecond per tensor), a tensor is looked at closely only where a sweep finds one."""
+    """-> (addresses, lengths, types, whether all are contiguous) of a list.  Nearly always all are, and a list has hundreds: each property is
+    asked for in one sweep (a microsecond per tensor), a tensor is looked at closely only where a sweep finds one."""
     try:
-        plain = all(map(_T.is_contiguous, tensors)) and not any(map(_T.is_neg, tensors)) and set(map(_LAYOUT, tensors)) <= {torch.strided}
+        plain = all(map(_T.is_contiguous, tensors))
+        fine = not any(map(_T.is_neg, tensors)) and set(map(_LAYOUT, tensors)) <= {torch.strided}
         types = [DTYPES[d] for d in map(_DTYPE, tensors)]
     except (TypeError, KeyError, RuntimeError):
-        plain, types = False, None
-    if not plain:
+        fine = False
+    if not fine:
         for i, t in enumerate(tensors):
-            _check_dense(t, f"{name} {i}")
-        types = [DTYPES[t.dtype] for t in tensors]
+            _check_tensor(t, f"{name} {i}")
+        raise _lib.NiwError(f"{name}: tensors whose layout cannot be read")
     return list(map(_T.data_ptr, tensors)), list(map(_T.numel, tensors)), types, plain
 
 
-def _check_pairs(first, second, name):
-    """the elements of a pair lie in the same order: both contiguous (of whatever shapes), or laid out alike"""
-    for i, (a, b) in enumerate(zip(first, second)):
-        if a.numel() != b.numel() or not (a.is_contiguous() and b.is_contiguous() or a.numel() < 2 or (a.shape == b.shape and _layout(a) == _layout(b))):
-            raise _lib.NiwError(f"{name} {i}: shape {tuple(b.shape)} strides {b.stride()} against {tuple(a.shape)} {a.stride()}; the elements of a pair have to "
-                                "lie in the same order")
+def _runs(tensors, name):
+    """The elements of equally shaped tensors that belong together, as gap-free stretches of memory that all of them share: -> (length of a
+    stretch, addresses of its beginnings per tensor).  One stretch for tensors that are dense in the same order, whatever that order is;
+    one per row for a slice of columns; the same address again where a dimension is expanded."""
+    first = tensors[0]
+    for t in tensors[1:]:
+        if t.shape != first.shape:
+            raise _lib.NiwError(f"{name}: shape {tuple(t.shape)} against {tuple(first.shape)}; tensors that are not all contiguous have to agree in shape")
+    dims = sorted((d for d, n in enumerate(first.shape) if n != 1), key=lambda d: -first.stride(d) or -math.inf)      # expanded ones outermost
+    length, k = 1, len(dims)
+    while k and all(t.stride(dims[k - 1]) == length for t in tensors):
+        k -= 1
+        length *= first.shape[dims[k]]
+    outer = dims[:k]
+    count = math.prod(first.shape[d] for d in outer)
+    if first.numel() and count > MAX_RUNS:
+        raise _lib.NiwError(f"{name}: shape {tuple(first.shape)} with strides {', '.join(str(t.stride()) for t in tensors)} falls into {count} stretches of "
+                            f"{length} elements (at most {MAX_RUNS}); pass dense tensors that lie in the same order")
+    begins = []
+    for t in tensors:
+        at = np.zeros(1, np.int64)
+        for d in outer:
+            at = (at[:, None] + np.arange(first.shape[d], dtype=np.int64) * t.stride(d)).reshape(-1)
+        begins.append(np.uint64(t.data_ptr()) + (at * t.element_size()).astype(np.uint64))
+    return length, begins
 
 
 def _check_device(tensors, name):
@@ -354,6 +364,29 @@ def _check_device(tensors, name):
 _GRAD_ROW = np.dtype([("grad", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("out_dtype", "<i4")])
 _ADAM_ROW = np.dtype([("param", "<u8"), ("grad", "<u8"), ("exp_avg", "<u8"), ("exp_avg_sq", "<u8"), ("master", "<u8"), ("n", "<i8"), ("param_dtype", "<i4"),
                       ("grad_dtype", "<i4"), ("group", "<i4"), ("reserved", "<i4")])
+
+
+def _rows(row, cols, pointers, plain, tensors, name):
+    """the rows of a list from its columns: one per entry, or one per stretch of the entries whose tensors are not all contiguous and of one
+    length.  pointers: the columns that are addresses, tensors: what they are the addresses of, one list per column"""
+    rows = np.zeros(len(cols["n"]), row)
+    for key, values in cols.items():
+        rows[key] = values
+    if plain:
+        return rows
+    count, split = np.ones(len(rows), np.int64), {}
+    for i in range(len(rows)):
+        some = [(key, t[i]) for key, t in zip(pointers, tensors) if t[i] is not None]
+        if any(not t.is_contiguous() or t.numel() != some[0][1].numel() for _, t in some):
+            length, begins = _runs([t for _, t in some], f"{name} {i}")
+            count[i], split[i] = len(begins[0]), (length, zip([key for key, _ in some], begins))
+    rows, end = np.repeat(rows, count), np.cumsum(count)
+    for i, (length, begins) in split.items():
+        here = slice(end[i] - count[i], end[i])
+        rows["n"][here] = length
+        for key, at in begins:
+            rows[key][here] = at
+    return rows
 
 
 _HERE = contextlib.nullcontext()
@@ -404,9 +437,10 @@ class _Table:
 class TensorTable(_Table):
     """What grad_norm / grad_total / clip_grads need to know of a list of tensors, gathered and checked once for tensors that stay where they
     are (a gradient bucket's views, gradients that are zeroed rather than dropped).  A plain list in its place is gathered at every call.
-    tensors: float32 / bfloat16 / float16, mixed at will, each dense in any order, any length; None entries are left out.
-    out: for clip_grads, one tensor per entry that receives the clipped values, of any of the types (as many elements in the same order: both
-    contiguous, of whatever shapes, or laid out alike); None: in place.
+    tensors: float32 / bfloat16 / float16, mixed at will, of any length and strides; None entries are left out.  Tensors that are not dense are
+    walked stretch by stretch (a slice of columns: row by row), up to MAX_RUNS of them.
+    out: for clip_grads, one tensor per entry that receives the clipped values, of any of the types (both contiguous with as many elements, or
+    of the same shape); None: in place.
     The table speaks of the MEMORY the tensors had when it was built and keeps that memory alive; a tensor that is given other storage
     afterwards (.grad re-created by a backward, .data re-assigned, .to()) is not followed: build a new table.  Building one waits for the GPU
     once; any stream, thread or captured graph may use it then, several at a time (a graph does not keep it alive: the caller does)."""
@@ -422,18 +456,16 @@ class TensorTable(_Table):
         given = sum(o is not None for o in out)
         if given not in (0, len(out)):
             raise _lib.NiwError("TensorTable: an output for some tensors only")
-        rows = np.zeros(len(tensors), _GRAD_ROW)
-        rows["grad"], lengths, rows["dtype"], plain = _gather(tensors, "tensor")
-        rows["n"], every = lengths, tensors
+        cols, every = {}, tensors
+        cols["grad"], cols["n"], cols["dtype"], plain = _gather(tensors, "tensor")
         if given:
-            rows["out"], out_lengths, rows["out_dtype"], out_plain = _gather(out, "output")
-            if lengths != out_lengths or not (plain and out_plain):
-                _check_pairs(tensors, out, "output")
-            every = tensors + out
+            cols["out"], lengths, cols["out_dtype"], out_plain = _gather(out, "output")
+            plain, every = plain and out_plain and lengths == cols["n"], tensors + out
         else:
-            rows["out"], rows["out_dtype"] = rows["grad"], rows["dtype"]
+            cols["out"], cols["out_dtype"] = cols["grad"], cols["dtype"]
+        rows = _rows(_GRAD_ROW, cols, ("grad", "out"), plain, (tensors, out if given else tensors), "tensor")
         self.device = _check_device(every, "TensorTable")
-        self.numel = sum(lengths)
+        self.numel = sum(cols["n"])
         kept = TABLE_KEPT if _kept else 0
         self._unclippable = None
         try:
@@ -525,7 +557,7 @@ class AdamTable(_Table):
         grads       float32 / bfloat16 / float16; a None entry leaves its parameter out
         exp_avg, exp_avg_sq     float32
         master      float32 copies that the update runs on (half-precision parameters receive the rounded result), None for float32
-    The tensors of one entry have as many elements in the same order in memory (all contiguous, of whatever shapes, or laid out alike)."""
+    The tensors of one entry are all contiguous with as many elements, or of the same shape with any strides."""
 
     def __init__(self, groups, _kept=True):
         groups = [dict(g) for g in groups]
@@ -549,29 +581,28 @@ class AdamTable(_Table):
             master += [lists["master"][i] for i in keep]
             group += [k] * len(keep)
         masters = [t for t in master if t is not None]
-        rows = np.zeros(len(group), _ADAM_ROW)
-        rows["group"], rows["master"] = group, 0
-        plain, lengths, types = {}, {}, {}
-        for field, key in zip(("param", "grad", "exp_avg", "exp_avg_sq"), names):
-            rows[field], lengths[key], types[key], plain[key] = _gather(cols[key], key)
-        own, _, types["master"], plain["master"] = _gather(masters, "master")
+        fields = ("param", "grad", "exp_avg", "exp_avg_sq")
+        columns, plain, types, lengths = dict(group=group), True, {}, None
+        for field, key in zip(fields, names):
+            columns[field], n, types[key], contiguous = _gather(cols[key], key)
+            lengths = n if lengths is None else lengths
+            plain = plain and contiguous and n == lengths
+        own, n, types["master"], contiguous = _gather(masters, "master")
+        plain = plain and contiguous and n == [m for m, w in zip(lengths, master) if w is not None]
         for key in names[2:] + ("master",):
             if any(types[key]):
                 raise _lib.NiwError(f"AdamTable: {key}: expected float32, got {next(t.dtype for t in cols.get(key, masters) if t.dtype != torch.float32)}")
-        with_master = [w is not None for w in master]
-        if [bool(t) for t in types["params"]] != with_master:
+        if [bool(t) for t in types["params"]] != [w is not None for w in master]:
             raise _lib.NiwError("AdamTable: a half-precision parameter needs a float32 master copy (updates below half a step of its type would be "
                                 "lost), a float32 parameter has none")
-        for key in names[1:]:
-            if lengths[key] != lengths["params"] or not (plain[key] and plain["params"]):
-                _check_pairs(cols["params"], cols[key], key)
-        _check_pairs([p for p, w in zip(cols["params"], master) if w is not None], masters, "master")
-        rows["master"][np.array(with_master, dtype=bool)] = own
-        rows["n"], rows["param_dtype"], rows["grad_dtype"] = lengths["params"], types["params"], types["grads"]
+        own = iter(own)
+        columns["master"] = [0 if w is None else next(own) for w in master]
+        columns["n"], columns["param_dtype"], columns["grad_dtype"] = lengths, types["params"], types["grads"]
+        rows = _rows(_ADAM_ROW, columns, fields + ("master",), plain, [cols[key] for key in names] + [master], "entry")
         tensors = [t for key in names for t in cols[key]] + masters
         self.device = _check_device(tensors, "AdamTable")
         self.n_groups = len(groups)
-        self.numel = sum(lengths["params"])
+        self.numel = sum(lengths)
         self._build("niw_adam_table", rows, (self.n_groups, TABLE_KEPT if _kept else 0), tensors, _kept)
 
 

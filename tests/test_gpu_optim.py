@@ -568,3 +568,96 @@ def test_random_lists():
         c = coefficient(exact_norm(before), 1.0)
         for v, b in zip(views, before):
             check_clipped(v, b, c)
+
+
+# ------------------------------------------------------------------------------------------ tensors that are not dense
+def strided(shape, form, dtype=F32, seed=0):
+    """(tensor of random values, the memory it lies in): laid out otherwise than in order"""
+    turned, n = tuple(reversed(shape)), math.prod(shape)
+    if form == "dense":
+        whole = rand(n, dtype, seed=seed).view(shape)
+        return whole, whole
+    if form == "reversed":                                                                       # the first dimension innermost
+        whole = rand(n, dtype, seed=seed).view(turned)
+        return whole.permute(*range(len(shape) - 1, -1, -1)), whole
+    if form == "columns":
+        whole = rand(math.prod(shape[:-1]) * (2 * shape[-1] + 3), dtype, seed=seed).view(*shape[:-1], -1)
+        return whole[..., 2:2 + shape[-1]], whole
+    assert form == "rows"
+    whole = rand(2 * n, dtype, seed=seed).view(2 * shape[0], *shape[1:])
+    return whole[::2], whole
+
+
+FORMS = ["dense", "reversed", "columns", "rows"]
+SHAPES = [(7,), (129, 65), (1, 300), (300, 1), (3, 5, 130), (2, 40000)]
+
+
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_strided_and_expanded_tensors(dtype, kind):
+    t = [strided(s, f, dtype, seed=i)[0] for i, (s, f) in enumerate((s, f) for s in SHAPES for f in FORMS)]
+    t += [rand(65, dtype, seed=99).expand(40, 65), rand(1, dtype, seed=98).view(1, 1).expand(90, 70), rand(33, dtype).view(33, 1).expand(33, 5)]
+    check_norm(ops.grad_norm(t, norm_type=kind), t, kind)
+    check_norm(ops.grad_norm(ops.TensorTable(t), norm_type=kind), t, kind)
+
+
+@pytest.mark.parametrize("out_form", [None] + FORMS)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, F32), (BF16, F32), (F16, F16)], ids=str)
+def test_clip_of_strided_tensors(form, out_form, dtype, out_dtype):
+    pairs = [strided(s, form, dtype, seed=i) for i, s in enumerate(SHAPES)]
+    g, before, whole = [p[0] for p in pairs], [p[0].clone() for p in pairs], [p[1].clone() for p in pairs]
+    outs = None if out_form is None else [strided(s, out_form, out_dtype, seed=50 + i) for i, s in enumerate(SHAPES)]
+    around = pairs if outs is None else outs
+    kept = [p[1].clone() for p in around]
+    want = exact_norm(before)
+    norm = ops.clip_grads(g, want / 3, out=None if outs is None else [o[0] for o in outs])
+    check_norm(norm, before)
+    for i, (o, memory) in enumerate(around):
+        check_clipped(o, before[i], coefficient(want, want / 3))
+        o.zero_()                                                            # what lies between the elements is as it was
+        view = kept[i].as_strided(o.shape, o.stride(), o.storage_offset() - memory.storage_offset())
+        view.zero_()
+        assert torch.equal(memory, kept[i])
+    assert outs is None or all(torch.equal(p[1], w) for p, w in zip(pairs, whole))
+
+
+def test_clip_of_shared_elements_is_refused_their_norm_is_not():
+    for g in (rand(6).expand(4, 6), rand(40).as_strided((5, 4), (3, 1))):
+        check_norm(ops.grad_norm([g]), [g])
+        with pytest.raises(_lib.NiwError, match="overlap"):
+            ops.clip_grads([g], 1.0)
+        out = torch.empty(g.shape, device=DEV)
+        before = g.clone()
+        ops.clip_grads([g], 0.5, out=[out])
+        check_clipped(out, before, coefficient(exact_norm([before]), 0.5))
+        with pytest.raises(_lib.NiwError, match="overlap"):
+            ops.clip_grads([out], 0.5, out=[g])
+
+
+@pytest.mark.parametrize("pt,gt", [(F32, F32), (BF16, BF16), (F16, F32)], ids=str)
+@pytest.mark.parametrize("forms", [("columns", "dense", "dense", "dense", "dense"), ("dense", "reversed", "dense", "dense", "dense"), ("reversed",) * 5,
+                                   ("rows", "columns", "reversed", "dense", "columns"), ("dense", "expanded", "dense", "rows", "dense")], ids="-".join)
+def test_adam_of_strided_tensors(pt, gt, forms):
+    shapes, s = [(129, 65), (3, 5, 70), (2, 20000)], dict(params=[], grads=[], exp_avg=[], exp_avg_sq=[], master=None if pt == F32 else [])
+    for i, shape in enumerate(shapes):
+        p = strided(shape, forms[0], pt, seed=10 * i)[0]
+        s["params"].append(p)
+        s["grads"].append(rand(shape[-1], gt, seed=10 * i + 1).expand(shape) if forms[1] == "expanded" else strided(shape, forms[1], gt, seed=10 * i + 1)[0])
+        s["exp_avg"].append(strided(shape, forms[2], F32, seed=10 * i + 2)[0])
+        s["exp_avg_sq"].append(strided(shape, forms[3], F32, seed=10 * i + 3)[0].square_())
+        if pt != F32:
+            s["master"].append(strided(shape, forms[4], F32, seed=10 * i + 4)[0].copy_(p))
+    before = copy_state(s)
+    want = exact_norm(before["grads"])
+    norm = ops.adam_step_tensors([s], lr=1e-2, step=4, weight_decay=0.1, max_norm=want / 2)
+    check_norm(norm, before["grads"])
+    check_adam(s, before, coefficient(want, want / 2), 1e-2, 4, 0.1)
+
+
+def test_adam_refuses_shared_elements_that_it_writes():
+    for key in ("params", "exp_avg", "exp_avg_sq"):
+        s = {k: [rand(24, seed=i).view(4, 6).square_()] for i, k in enumerate(("params", "grads", "exp_avg", "exp_avg_sq"))}
+        s[key] = [rand(6).expand(4, 6)]
+        with pytest.raises(_lib.NiwError, match="overlap"):
+            ops.AdamTable([s])

@@ -3,6 +3,7 @@ Python wrappers.  Nothing is launched: every check runs on the host, in front of
 import ctypes
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -204,14 +205,14 @@ def z(*shape, dtype=torch.float32):
     ([z(4, dtype=torch.float64)], None, "float64"),
     ([z(4, dtype=torch.int32)], None, "int32"),
     ([3.0], None, "float"),
-    ([z(8)[::2]], None, "gaps"),
-    ([z(1, 4).expand(3, 4)], None, "shares"),
-    ([z(4, 6)[:, :3]], None, "gaps"),
+    ([z(600000)[::2]], None, "300000 stretches of 1 elements"),
+    ([z(600, 500).t()], [z(500, 600)], "300000 stretches of 1 elements"),
     ([z(4).to_sparse()], None, "sparse"),
     ([z(4)], [], "1 tensors and 0 outputs"),
     ([z(4), z(4)], [z(4), None], "some tensors only"),
-    ([z(4)], [z(5)], "same order"),
-    ([z(4, 6)], [z(6, 4).t()], "same order"),
+    ([z(4)], [z(5)], "agree in shape"),
+    ([z(4, 6)], [z(4, 6).t()], "agree in shape"),
+    ([z(8)[::2]], [z(2, 2)], "agree in shape"),
     ([z(4)], [z(4, dtype=torch.int64)], "int64"),
     ([torch._neg_view(z(4))], None, "negated"),
     ([z(4)], None, "expected CUDA/HIP"),
@@ -227,6 +228,79 @@ def test_rows_of_a_list_have_the_layout_of_the_descriptors():
     for row, struct in ((ops._GRAD_ROW, _lib.GradTensor), (ops._ADAM_ROW, _lib.AdamTensor)):
         assert row.itemsize == ctypes.sizeof(struct)
         assert [(n, row.fields[n][1]) for n in row.names] == [(n, getattr(struct, n).offset) for n, _ in struct._fields_]
+
+
+def strided(shape, form, dtype=torch.float32):
+    """a tensor of that shape, laid out otherwise than in order"""
+    n = len(shape)
+    if form == "dense":
+        return torch.empty(shape, dtype=dtype)
+    if form == "reversed":                                                                       # the first dimension innermost
+        return torch.empty(shape[::-1], dtype=dtype).permute(*range(n - 1, -1, -1))
+    if form == "columns":
+        return torch.empty((*shape[:-1], 2 * shape[-1] + 3), dtype=dtype)[..., 2:2 + shape[-1]]
+    if form == "rows":
+        return torch.empty((2 * shape[0], *shape[1:]), dtype=dtype)[::2]
+    assert form == "expanded"
+    return torch.empty((1, *shape[1:]), dtype=dtype).expand(shape)
+
+
+FORMS = ["dense", "reversed", "columns", "rows", "expanded"]
+
+
+def addresses(t):
+    """of every element, in the order of its index"""
+    at = np.zeros(t.shape, np.int64)
+    for d, n in enumerate(t.shape):
+        at += (np.arange(n) * t.stride(d)).reshape([-1 if k == d else 1 for k in range(t.dim())])
+    return (t.data_ptr() + at * t.element_size()).reshape(-1)
+
+
+@pytest.mark.parametrize("second", FORMS)
+@pytest.mark.parametrize("first", FORMS)
+@pytest.mark.parametrize("shape", [(1,), (7,), (5, 6), (1, 6), (5, 1), (3, 4, 5), (2, 1, 3, 4), (0, 4), (4, 0)])
+def test_stretches_pair_the_elements_that_belong_together(shape, first, second):
+    """over all stretches, the pairs of addresses walked are those of the elements of equal index, each once"""
+    a, b = strided(shape, first), strided(shape, second, torch.bfloat16)
+    length, (at, to) = ops._runs([a, b], "pair")
+    walked = [(int(x) + 4 * j, int(y) + 2 * j) for x, y in zip(at, to) for j in range(length)]
+    assert sorted(walked) == sorted(zip(addresses(a).tolist(), addresses(b).tolist()))
+
+
+@pytest.mark.parametrize("form,length,count", [("dense", 120, 1), ("reversed", 120, 1), ("columns", 6, 20), ("rows", 30, 4), ("expanded", 30, 4)])
+def test_stretches_are_as_long_as_the_layout_allows(form, length, count):
+    got, (at,) = ops._runs([strided((4, 5, 6), form)], "tensor")
+    assert (got, len(at)) == (length, count)
+
+
+def test_rows_of_a_mixed_list():
+    """entries in step keep one row, the others have one per stretch, in the entries' order"""
+    t = [z(5), z(3, 8)[:, 2:6], z(0), z(4, 6).t(), z(0, 4)[:, 1:3], z(6)]
+    out = [z(5), z(3, 4), z(0), z(4, 6).t(), z(0, 2), z(2, 3)]
+    cols = dict(grad=[x.data_ptr() for x in t], out=[x.data_ptr() for x in out], n=[x.numel() for x in t], dtype=0, out_dtype=0)
+    rows = ops._rows(ops._GRAD_ROW, cols, ("grad", "out"), False, (t, out), "tensor")
+    assert [int(n) for n in rows["n"] if n] == [5, 4, 4, 4, 24, 6]
+    full = rows[rows["n"] > 0]
+    assert full["grad"].tolist() == [t[0].data_ptr()] + [t[1].data_ptr() + 32 * k for k in range(3)] + [t[3].data_ptr(), t[5].data_ptr()]
+    assert full["out"].tolist() == [out[0].data_ptr()] + [out[1].data_ptr() + 16 * k for k in range(3)] + [out[3].data_ptr(), out[5].data_ptr()]
+
+
+@pytest.mark.parametrize("tensors,overlap", [
+    (lambda: [z(1, 4).expand(3, 4)], True), (lambda: [z(12).as_strided((3, 4), (2, 1))], True), (lambda: [z(4, 6)[:, :3]], False),
+    (lambda: (lambda x: [x[:, :3], x[:, 3:]])(z(4, 6)), False), (lambda: (lambda x: [x[:, :4], x[:, 3:]])(z(4, 6)), True),
+    (lambda: (lambda x: [x[::2], x[1::2]])(z(9)), False), (lambda: [z(6, 4).t()], False),
+])
+def test_written_stretches_that_overlap_are_refused(tensors, overlap):
+    """what has a norm need not be clippable in place: elements that several indices share would be scaled several times"""
+    t = tensors()
+    cols = dict(grad=[x.data_ptr() for x in t], out=[x.data_ptr() for x in t], n=[x.numel() for x in t], dtype=0, out_dtype=0)
+    rows = ops._rows(ops._GRAD_ROW, cols, ("grad", "out"), False, (t, t), "tensor")
+    lib, table = _lib.load(), _lib.Table()
+    image = np.zeros(lib.niw_table_bytes(len(rows)), np.uint8)
+    for flags, refused in ((0, False), (ops.TABLE_CLIP, overlap)):
+        code = lib.niw_grad_table(rows.ctypes.data, len(rows), flags, image.ctypes.data, ctypes.byref(table))
+        assert code == (-1 if refused else 0)
+        assert not refused or "overlap" in err()
 
 
 def test_none_entries_are_left_out_before_any_check():
@@ -257,9 +331,10 @@ def group(**kw):
     ([], "1..8 groups"), ([group()] * 9, "1..8 groups"),
     ([group(lr=[1.0])], "unknown keys"), ([group(grads=None)], "needs params"), ([group(grads=[])], "differ in length"),
     ([group(exp_avg=[z(4, dtype=torch.bfloat16)])], "expected float32"), ([group(params=[z(4, dtype=torch.bfloat16)])], "master copy"),
-    ([group(master=[z(4)])], "has none"), ([group(grads=[z(5)])], "same order"),
-    ([group(params=[z(2, 3)], grads=[z(3, 2).t()], exp_avg=[z(2, 3)], exp_avg_sq=[z(2, 3)])], "same order"),
-    ([group(params=[z(8)[::2]])], "gaps"), ([group()], "expected CUDA/HIP"), ([group(grads=[z(4, dtype=torch.float64)])], "float64"),
+    ([group(master=[z(4)])], "has none"), ([group(grads=[z(5)])], "agree in shape"),
+    ([group(params=[z(2, 3)], grads=[z(3, 2)], exp_avg=[z(2, 3)], exp_avg_sq=[z(2, 3).t()])], "agree in shape"),
+    ([group(params=[z(4, dtype=torch.bfloat16)], master=[z(5)])], "agree in shape"),
+    ([group(grads=[z(8)[::2]], exp_avg=[z(5)])], "agree in shape"), ([group()], "expected CUDA/HIP"), ([group(grads=[z(4, dtype=torch.float64)])], "float64"),
 ])
 def test_adam_table_refuses(groups, what):
     with pytest.raises(_lib.NiwError, match=what):
