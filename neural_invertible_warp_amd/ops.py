@@ -403,14 +403,14 @@ class _Table:
     """Device image of a list of tensors (niw_table).  The image is stored on the stream that is current when the table is built; a table that
     is kept (`kept`) waits for that once, so that any stream may use it afterwards."""
 
-    def _build(self, name, rows, how, tensors, kept):
+    def _build(self, name, rows, how, entries, tensors, kept):
         lib = _lib.load()
         self._keep = [tensors, [t.untyped_storage() for t in tensors]]
         host = np.empty(max(lib.niw_table_bytes(len(rows)), 16), np.uint8)
         image = ctypes.c_void_p(host.ctypes.data)
         self._c = _lib.Table()
         if getattr(lib, name)(ctypes.c_void_p(rows.ctypes.data), len(rows), *how, image, ctypes.byref(self._c)):
-            raise _lib.NiwError(lib.niw_last_error_string().decode())
+            raise _lib.NiwError(lib.niw_last_error_string().decode() + (f" (counting the stretches of a list of {entries})" if len(rows) != entries else ""))
         self._streams, self._image = set(), None
         if self._c.bytes:
             if kept and torch.cuda.is_current_stream_capturing():
@@ -469,12 +469,12 @@ class TensorTable(_Table):
         kept = TABLE_KEPT if _kept else 0
         self._unclippable = None
         try:
-            self._build("niw_grad_table", rows, (TABLE_CLIP | kept,), every, _kept)
+            self._build("niw_grad_table", rows, (TABLE_CLIP | kept,), len(tensors), every, _kept)
         except _lib.NiwError as e:
             if given or "overlap" not in str(e):
                 raise
             self._unclippable = str(e)               # tensors that share memory have a norm, but cannot be clipped in place
-            self._build("niw_grad_table", rows, (kept,), every, _kept)
+            self._build("niw_grad_table", rows, (kept,), len(tensors), every, _kept)
 
 
 def _table(grads, out=None):
@@ -603,7 +603,7 @@ class AdamTable(_Table):
         self.device = _check_device(tensors, "AdamTable")
         self.n_groups = len(groups)
         self.numel = sum(lengths)
-        self._build("niw_adam_table", rows, (self.n_groups, TABLE_KEPT if _kept else 0), tensors, _kept)
+        self._build("niw_adam_table", rows, (self.n_groups, TABLE_KEPT if _kept else 0), len(lengths), tensors, _kept)
 
 
 def _per_group(value, n, name, kind):

@@ -173,3 +173,33 @@ def test_torch_optimizers_see_clipped_gradients(args, tmp_path, capsys):
     # every gradient is off by half a step of the factor, of the product and of its own rounding at most: so is their norm
     want = 1e-3 * float(m.grad_norm) / (float(m.grad_norm) + 1e-6)
     assert abs(left - want) <= 4 * H * want
+
+
+def test_two_ranks_clip_by_the_norm_of_the_exchanged_gradients(tmp_path):
+    """two gloo ranks on this GPU, each with its share of the rays: both log the same norms -- that of the summed gradients -- and stay equal"""
+    import os
+    import re
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    args = ["--model=barf_inn_llff", "--yaml=barf_inn_llff", "--barf_c2f=[0.1,0.5]", "--loss_weight.global_alignment=2", "--data.dataset=synthetic",
+            "--data.image_size=[24,32]", "--nerf.rand_rays=288", "--nerf.sample_intvs=32", "--freq.val=2", "--freq.ckpt=100", "--freq.scalar=1",
+            "--optim.clip_norm=1e-3", "--optim.skip_nonfinite", f"--output_root={tmp_path}", "--name=clip", "--max_iter=4"]
+    procs = []
+    for rank in range(2):
+        env = dict(os.environ, MASTER_ADDR="127.0.0.1", MASTER_PORT="29677", RANK=str(rank), WORLD_SIZE="2", LOCAL_RANK="0", NIW_DIST_BACKEND="gloo")
+        procs.append(subprocess.Popen([sys.executable, "-m", "neural_invertible_warp_amd.train"] + args, cwd=root, env=env, stdout=subprocess.PIPE,
+                                      stderr=subprocess.PIPE, text=True))
+    try:
+        outs = [p.communicate(timeout=100) for p in procs]
+    finally:
+        for p in procs:
+            if p.poll() is None:
+                p.kill()
+    for p, (out, err) in zip(procs, outs):
+        assert p.returncode == 0, err[-2000:]
+    val = [[l for l in out.splitlines() if l.startswith("[val it 4]")] for out, _ in outs]
+    assert val[0] and val[0] == val[1], val
+    norms = [re.findall(r"grad_norm=(\S+)", out) for out, _ in outs]
+    assert len(norms[0]) >= 3 and norms[0] == norms[1]
+    assert all(math.isfinite(float(n)) and float(n) > 1e-3 for n in norms[0])

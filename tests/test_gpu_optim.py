@@ -625,7 +625,7 @@ def test_clip_of_strided_tensors(form, out_form, dtype, out_dtype):
 def test_clip_of_shared_elements_is_refused_their_norm_is_not():
     for g in (rand(6).expand(4, 6), rand(40).as_strided((5, 4), (3, 1))):
         check_norm(ops.grad_norm([g]), [g])
-        with pytest.raises(_lib.NiwError, match="overlap"):
+        with pytest.raises(_lib.NiwError, match="overlap.*stretches of a list of 1"):
             ops.clip_grads([g], 1.0)
         out = torch.empty(g.shape, device=DEV)
         before = g.clone()
