@@ -433,8 +433,9 @@ int niw_grad_norm(const niw_table* table, int kind, double* workspace, double* t
 int niw_grad_clip(const niw_table* table, int kind, double max_norm, const double* total, double* workspace, float* norm_out, niw_stream_t stream);
 
 /* Adam with decoupled weight decay over a list of tensors, under an optional clip by the global norm of its gradients: per element
- *     g = c * grad;  p -= lr * weight_decay * p;  then niw_adam_step's update of p, exp_avg, exp_avg_sq by g
- * (the same arithmetic, so that with c = 1 and no decay the two give the same bits).  The clipped gradient is never written.  A
+ *     g = c * grad;  p *= 1 - lr * weight_decay;  then niw_adam_step's update of p, exp_avg, exp_avg_sq by g
+ * (the same arithmetic, so that with c = 1 a group without decay gets the same bits, whatever the other groups' decay).  The decay is
+ * rounded once, as p - (lr * weight_decay) p; an infinite p stays infinite (NaN at lr * weight_decay = 1).  The clipped gradient is never written.  A
  * half-precision parameter is updated through its fp32 `master` copy and receives the rounded result. */
 #define NIW_ADAM_MAX_GROUPS 8
 typedef struct niw_adam_tensor {

@@ -406,7 +406,12 @@ struct AdamArgs {
 
 // The update, one part of 1024 elements per workgroup: four elements of every stream per thread, 28 to 30 bytes each, and nothing reused.
 // 335 M bf16 parameters with master copies 1489 us, 101 M fp32 with fp16 gradients in unaligned tensors 408 us.
-// DECAY: some group of the call decays (without, an infinite parameter is not multiplied by 0 either).
+// DECAY: some group of the call decays.  Which one is the workgroup's own question: a group whose decay is 0 is left out of it.
+// p (1 - decay) is formed as p - decay p in one fma, which keeps what 1 - decay would lose in fp32 (a decay of 1e-5 has three digits there, one
+// below 2^-25 none).  An infinite parameter has no p - decay p, and a zero loses its sign there: both take the product.
+__device__ __forceinline__ float decayed(float p, float decay) {
+    return p == 0.f || isinf(p) ? p * (1.f - decay) : fmaf(-decay, p, p);
+}
 template <int KIND, bool NT, bool DECAY>
 __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> list, AdamArgs a, Clip clip) {
     const Factor factor = clip_factor<KIND>(clip);
@@ -421,7 +426,7 @@ __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> l
         with_dtype((s.types >> 8) & 255, [&](auto pt) {
             constexpr int G = decltype(gt)::value, P = decltype(pt)::value;
             auto update = [&](float& p, float g, float& m, float& v) {
-                if constexpr (DECAY) p = fmaf(-decay, p, p);
+                if (DECAY && decay != 0.f) p = decayed(p, decay);
                 niw::adam_update(p, niw::mul_rn(factor.c, g), m, v, a.w1, a.b2, a.w2, a.eps, step_size, bc2_sqrt);
             };
             const long long odd = odd_element<4>(part.head, part.begin, part.end);
