@@ -185,12 +185,45 @@ __device__ __forceinline__ Part<Slot> part_of(const List<Slot>& list) {
 
 // ------------------------------------------------------------------------------------------------ elements
 // Vectors of four elements (16 bytes of fp32, 8 of the half types) that may begin on any element: the aligned(..) attributes promise the
-// compiler no more than that, and gfx950 takes such accesses as one instruction.
+// compiler no more than that, and gfx950 takes such accesses as one instruction.  (A template argument drops the attribute, so each
+// access names its type here: the build treats -Walign-mismatch, which reports the loss, as an error.)
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+// NT: past the caches (a list that does not fit them anyway leaves them to what does)
+template <bool NT>
+__device__ __forceinline__ f32x4 get_f4(const float* p) {
+    const f32x4_any* const q = reinterpret_cast<const f32x4_any*>(p);
+    if constexpr (NT) return __builtin_nontemporal_load(q);
+    else return *q;
+}
+template <bool NT>
+__device__ __forceinline__ u32x2 get_u2(const unsigned short* p) {
+    const u32x2_any* const q = reinterpret_cast<const u32x2_any*>(p);
+    if constexpr (NT) return __builtin_nontemporal_load(q);
+    else return *q;
+}
+template <bool NT>
+__device__ __forceinline__ u32x4 get_u4(const char* p) {
+    const u32x4_any* const q = reinterpret_cast<const u32x4_any*>(p);
+    if constexpr (NT) return __builtin_nontemporal_load(q);
+    else return *q;
+}
+template <bool NT>
+__device__ __forceinline__ void put_f4(float* p, f32x4 x) {
+    f32x4_any* const q = reinterpret_cast<f32x4_any*>(p);
+    if constexpr (NT) __builtin_nontemporal_store(x, q);
+    else *q = x;
+}
+template <bool NT>
+__device__ __forceinline__ void put_u2(unsigned short* p, u32x2 x) {
+    u32x2_any* const q = reinterpret_cast<u32x2_any*>(p);
+    if constexpr (NT) __builtin_nontemporal_store(x, q);
+    else *q = x;
+}
 
 template <int DT>
 __device__ __forceinline__ float widen(unsigned short bits) {
@@ -202,22 +235,11 @@ __device__ __forceinline__ float load1(const void* p, long long i) {
     if constexpr (DT == NIW_F32) return static_cast<const float*>(p)[i];
     else return widen<DT>(static_cast<const unsigned short*>(p)[i]);
 }
-// NT: past the caches (a list that does not fit them anyway leaves them to what does)
-template <bool NT, class V>
-__device__ __forceinline__ V get(const V* p) {
-    if constexpr (NT) return __builtin_nontemporal_load(p);
-    else return *p;
-}
-template <bool NT, class V, class X>
-__device__ __forceinline__ void put(V* p, X x) {
-    if constexpr (NT) __builtin_nontemporal_store((V)x, p);
-    else *p = x;
-}
 template <bool NT, int DT>
 __device__ __forceinline__ f32x4 load4(const void* p, long long i) {
-    if constexpr (DT == NIW_F32) return get<NT>(reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + i));
+    if constexpr (DT == NIW_F32) return get_f4<NT>(static_cast<const float*>(p) + i);
     else {
-        const u32x2 w = get<NT>(reinterpret_cast<const u32x2_any*>(static_cast<const unsigned short*>(p) + i));
+        const u32x2 w = get_u2<NT>(static_cast<const unsigned short*>(p) + i);
         return f32x4{widen<DT>((unsigned short)w[0]), widen<DT>((unsigned short)(w[0] >> 16)), widen<DT>((unsigned short)w[1]), widen<DT>((unsigned short)(w[1] >> 16))};
     }
 }
@@ -237,8 +259,8 @@ __device__ __forceinline__ void store1(void* p, long long i, float x) {
 }
 template <bool NT, int DT>
 __device__ __forceinline__ void store4(void* p, long long i, f32x4 x) {
-    if constexpr (DT == NIW_F32) put<NT>(reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + i), x);
-    else put<NT>(reinterpret_cast<u32x2_any*>(static_cast<unsigned short*>(p) + i), u32x2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])});
+    if constexpr (DT == NIW_F32) put_f4<NT>(static_cast<float*>(p) + i, x);
+    else put_u2<NT>(static_cast<unsigned short*>(p) + i, u32x2{narrow2<DT>(x[0], x[1]), narrow2<DT>(x[2], x[3])});
 }
 // f(std::integral_constant dtype) for the dtype of a descriptor: the branch is the same for a whole workgroup
 template <class F>
@@ -285,7 +307,7 @@ template <int KIND, int DT, bool NT>
 __device__ __forceinline__ void see(Seen<KIND>& seen, const void* p, int head, long long begin, long long end) {
     constexpr int V = DT == NIW_F32 ? 4 : 8, U = 4;      // 16 bytes per thread and load, U loads under way
     const int tid = threadIdx.x;
-    auto words = [&](long long i) { return get<NT>(reinterpret_cast<const u32x4_any*>(static_cast<const char*>(p) + i * (16 / V))); };
+    auto words = [&](long long i) { return get_u4<NT>(static_cast<const char*>(p) + i * (16 / V)); };
     auto take = [&](u32x4 w) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
