@@ -23,11 +23,10 @@ B x R rays); `strong` keeps the reference's GLOBAL batch (4096 / 2048 rays) and 
 on one GPU: a proxy of what one rank of a K-GPU strong-scaled job executes (no collective).  Prints ONE JSON line on rank 0.
 
 An iteration is ONE library call (niw_train_step: forward, losses, backward of every stage, 25 launches) + the gradient all-reduce
-(N > 1) + ONE Adam launch.  At N = 1 the timed iterations replay a captured HIP graph of it (the step's scalars -- c2f bands, warp
-windows, Adam bias corrections, pixel-draw number -- travel in a 256-byte device buffer refreshed before every replay); under N > 1
-the default is launch by launch, which since round 4 is the FASTER form at every size (the host needs ~0.3 ms per iteration, a rank's
-1/8 share of cfg3 takes 1.0 ms: measured 1.005 ms launched, 1.023 ms replayed).  `--hip-graph on` under N > 1 captures two graphs around
-the eagerly issued RCCL all-reduce; should the capture fail, the rank says so in a marker file and exits, and the launcher parent --
+(N > 1) + ONE Adam launch, launched at every N: the FASTER form at every size (the host needs ~0.3 ms per iteration, a rank's 1/8 share of
+cfg3 takes 1.0 ms: measured 1.005 ms launched, 1.023 ms replayed as a HIP graph).  `--hip-graph on` is refused while engine.REPLAY_OFF stands
+(a replayed train iteration has ended processes for a reason that is not known); what follows it is kept for then: two graphs around
+the eagerly issued RCCL all-reduce under N > 1; should the capture fail, the rank says so in a marker file and exits, and the launcher parent --
 which never touched the GPU -- starts a fresh set of ranks with `--hip-graph off` (a failed capture is not recoverable in-process).
 
 N > 1 prints ONE line holding both scaling modes: the weak-scaled step is the headline (`value`, `ms_per_step`: 4096 / 2048 rays per
@@ -329,7 +328,7 @@ def scenes_of_rank(scenes, rank, world):
     return [sc for i, sc in enumerate(scenes) if i % world == rank]
 
 
-def build_workloads(name, dev, rank, world, scaling, shard_of, hip_graph=True, precision="fp32", overlap=True, placement="shard", llff_root=None,
+def build_workloads(name, dev, rank, world, scaling, shard_of, hip_graph=False, precision="fp32", overlap=True, placement="shard", llff_root=None,
                     split_exchange="auto", fused_step="auto"):
     """-> (list of (trainer, var0, B, R_local, S, Sf), description).  placement (cfg4, all scenes): "shard" = every rank trains every scene on
     its share of the rays (gradient all-reduce per scene and step); "replicas" = scene i trains WHOLE on rank i mod N, no exchange at all
@@ -482,9 +481,8 @@ def main():
     ap.add_argument("--no-torch-baseline", action="store_true", help="skip the oracle's step under PyTorch-ROCm on this GPU (torch_rocm_baseline)")
     ap.add_argument("--lean", action="store_true", help="train step only: all four --no-* switches")
     ap.add_argument("--hip-graph", choices=["auto", "on", "off"], default="auto",
-                    help="replay the captured HIP graph of the iteration (on) or launch it call by call (off); auto = on for one GPU, off under "
-                         "torch.distributed (round 4: launched is the faster form at every size, also for a 1/8 share -- 1.005 vs 1.023 ms).  With "
-                         "`on` under N > 1 a failed capture makes the launcher parent start fresh ranks with `off`")
+                    help="replay the captured HIP graph of the iteration (on: refused while engine.REPLAY_OFF stands) or launch it call by call "
+                         "(off, auto: the faster form at every size, also for a 1/8 share -- 1.005 vs 1.023 ms)")
     ap.add_argument("--no-hip-graph", action="store_true", help="same as --hip-graph off")
     ap.add_argument("--kernel-steps", type=int, default=3, help="extra eager steps after the timed region for the per-kernel device-event table (0: skip)")
     ap.add_argument("--precision", choices=["fp32", "bf16x3", "bf16"], default="fp32",
@@ -546,7 +544,9 @@ def main():
     scaling = args.scaling or ("strong" if args.shard_of else "weak")
 
     from neural_invertible_warp_amd import engine
-    use_graph = False if args.no_hip_graph else ((world == 1 and not args.force_dist) if args.hip_graph == "auto" else args.hip_graph == "on")
+    use_graph = args.hip_graph == "on" and not args.no_hip_graph
+    if use_graph and engine.REPLAY_OFF:
+        raise SystemExit(f"bench.py: {engine.REPLAY_OFF}")
     exact = args.precision == "fp32"
     peak_mfma = PEAK_FP32_MFMA if exact else PEAK_BF16_MFMA
     n_evals = lambda loads_: sum(int(round(B * R)) * (S + (S + Sf if Sf else 0)) for _, _, B, R, S, Sf in loads_)
@@ -840,10 +840,14 @@ def main():
                             "captures cannot be agreed on host-side, so the replayed leg is not attempted")
             loads_g = []
         else:
-            loads_g, _ = build_workloads(args.config, dev, rank, world, scaling, 0, placement="shard", **dict(wl_ab, hip_graph=True))
-            guard_captures(loads_g, "ab_graph")
+            try:
+                loads_g, _ = build_workloads(args.config, dev, rank, world, scaling, 0, placement="shard", **dict(wl_ab, hip_graph=True))
+                guard_captures(loads_g, "ab_graph")
+            except engine.NiwError as e:                        # (refused on every rank alike, before any of them touched the device)
+                loads_g = []
+                graph_ab = dict(launched_ms=off["ms"], replayed_ms=None, capture_failed=str(e))
         try:
-            if not store_ok:
+            if not loads_g:
                 raise StopIteration
             rep = leg(loads_g)
             graph_ab = dict(launched_ms=off["ms"], replayed_ms=rep["ms"] if rep["hip_graph"] else None, replayed=rep, steps=args.steps,

@@ -27,6 +27,13 @@ class CaptureError(NiwError):
     starts a fresh process with hip_graph=False (bench.py does)"""
 
 
+# Replay of captured train iterations is switched off.  Two runs of all GPU tests in one process ended in a segmentation fault of the host: the
+# first inside CUDAGraph.replay() of a trainer, the second among the same file's tests (its kept output does not name one).  No GPU fault was
+# reported and the cause is not known, so INNTrainer refuses hip_graph=True until it is; the launched iteration is as fast.
+REPLAY_OFF = ("hip_graph=True is switched off: replaying a captured train iteration has ended processes with a segmentation fault on the host whose "
+              "cause is not known; run launched (hip_graph=False, bench.py --hip-graph off), which is as fast")
+
+
 class StepConstants:
     """Every step-dependent SCALAR of a train iteration in one small device buffer, refreshed by one host-to-device copy per step:
     c2f band weights (10 + 4), the warp's annealing windows (6 + 6), the two step-dependent Adam scalars of every optimizer group
@@ -388,9 +395,9 @@ class INNTrainer:
     def __init__(self, opt, n_views, rank=0, world=1, warp_perturb=0.0, seed=0, initial_poses_w2c=None, ray_sampler=None, hip_graph=False,
                  fused_step="auto", overlap=True, split_exchange="auto", collectives=True):
         """ray_sampler: "feistel" (one sort-free launch, default on the GPU) or "randperm" (the reference's torch.randperm call).
-        hip_graph: capture the whole iteration (forward, backward, gradient gather, Adam) into a HIP graph after two eager
-        steps and replay it from then on -- one graph launch + one 256-byte constants upload per step instead of ~140 launches;
-        needs inputs that stay at the same device addresses from step to step (the engine's resident `var` tensors do).
+        hip_graph: refused while REPLAY_OFF stands (NiwError).  What it did and will do: capture the whole iteration (forward, backward,
+        gradient gather, Adam) into a HIP graph after two eager steps and replay it from then on; needs inputs that stay at the same
+        device addresses from step to step (the engine's resident `var` tensors do).
         fused_step: "auto" (default) runs the iteration as one niw_train_step call (FusedStep) wherever that call covers the
         configuration and through the autograd mirror elsewhere; True insists (NiwError otherwise); False = always the mirror.
         split_exchange (ranks > 1, a fine network present): the gradient exchange as TWO all-reduces -- the fine network's segment,
@@ -400,6 +407,8 @@ class INNTrainer:
         one flat all-reduce (rounds 1-4).  Same sums either way.
         collectives=False: this trainer is a REPLICA (one scene per GPU, bench.py --placement replicas): it never exchanges anything,
         whatever process group is live."""
+        if hip_graph and REPLAY_OFF:
+            raise NiwError(REPLAY_OFF)
         self.opt, self.rank, self.world, self.n_views = opt, rank, world, n_views
         o = opt.optim
         if o.get("algo", "Adam") != "Adam":

@@ -19,8 +19,34 @@ def pytest_configure(config):
         torch.utils.deterministic.fill_uninitialized_memory = True
 
 
+# Tests that replay a trainer's captured iteration: skipped while engine.REPLAY_OFF stands.  Two runs of all GPU tests ended in a segmentation fault
+# of the host, the first inside CUDAGraph.replay() of such a trainer; no GPU fault was reported and the cause is not known.
+# (tests/test_gpu_launched.py runs the launched halves of those that had one.)
+REPLAYS_A_TRAINER = {
+    "test_gpu_clip_training.py": ["test_captured_iterations_clip_like_launched_ones"],
+    "test_gpu_fused_step.py": ["test_fused_iteration_with_and_without_the_second_stream", "test_fused_iteration_captured_graph_equals_eager",
+                               "test_captured_iteration_survives_sync_state_under_ray_sharding",
+                               "test_captured_iteration_with_density_noise_draws_a_fresh_stream_every_replay"],
+    "test_gpu_ranks.py": ["test_a_failed_capture_on_one_rank_costs_the_field_not_the_line"],
+    "test_gpu_sharding.py": ["test_bench_line_through_a_live_rccl_group_eager_and_captured"],
+    "test_gpu_step_ops.py": ["test_hip_graph_replay_equals_eager_training", "test_hip_graph_replay_equals_eager_at_full_batch_size",
+                             "test_hip_graph_replays_without_host_synchronisation_use_their_own_step_constants",
+                             "test_hip_graph_capture_after_a_resume_at_a_late_iteration",
+                             "test_eval_render_under_hip_graph_uses_the_host_bands_not_the_step_buffer",
+                             "test_hip_graph_replay_refuses_or_refreshes_inputs_it_was_not_captured_with",
+                             "test_training_is_bit_reproducible_and_graph_replay_equals_eager_bit_for_bit"],
+}
+
+
 def pytest_collection_modifyitems(config, items):
     import torch
+    from neural_invertible_warp_amd import engine
+    if engine.REPLAY_OFF:
+        replay = pytest.mark.skip(reason="replays a trainer's captured iteration, which is switched off: it has ended processes with a segmentation fault "
+                                         "on the host whose cause is not known (engine.REPLAY_OFF)")
+        for item in items:
+            if getattr(item, "originalname", item.name) in REPLAYS_A_TRAINER.get(os.path.basename(str(item.fspath)), ()):
+                item.add_marker(replay)
     if torch.cuda.is_available():
         return
     skip = pytest.mark.skip(reason="no GPU visible")
