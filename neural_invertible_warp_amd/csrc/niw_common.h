@@ -174,6 +174,11 @@ __device__ __forceinline__ float sub_rn(float a, float b) {
     return a - b;
 }
 
+// length of a ray as the unit view direction divides by it (nerf.py:452): what is fused is stated, so that forward and backward round alike
+__device__ __forceinline__ float ray_length(float x, float y, float z) {
+    return fmaxf(sqrtf(add_rn(fmaf(y, y, mul_rn(x, x)), mul_rn(z, z))), 1e-12f);
+}
+
 // sin / cos of the band argument fl32(x * 2^k * pi32).
 // The reference evaluates sin(fl32(x * f_k)) with f_k = 2^k * fl32(pi) (nerf.py:478-480; the warp's embedder alike:
 // model/nvp/embedder.py:26-32).  Scaling by a

@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256, 1) void mlp_bwd_dx_kernel(MlpBwdArgs a) {
     const long long ri = mc / a.S;
     const float d = a.depth[mc];
     const float rx = a.ray[ri * 3], ry = a.ray[ri * 3 + 1], rz = a.ray[ri * 3 + 2];
-    const float nrm = fmaxf(sqrtf(rx * rx + ry * ry + rz * rz), 1e-12f);
+    const float nrm = ray_length(rx, ry, rz);
     const float ux = rx / nrm, uy = ry / nrm, uz = rz / nrm;
     const float dot = ux * du[0] + uy * du[1] + uz * du[2];
     float gc[3] = {dp[0], dp[1], dp[2]};

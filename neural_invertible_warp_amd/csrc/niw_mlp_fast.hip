@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256, 1) void mlp_fwd_fast_kernel(FastFwdArgs a) {
         p[0] = add_rn(a.center[ri * 3 + 0], mul_rn(rx, d));
         p[1] = add_rn(a.center[ri * 3 + 1], mul_rn(ry, d));
         p[2] = add_rn(a.center[ri * 3 + 2], mul_rn(rz, d));
-        const float nrm = fmaxf(sqrtf(rx * rx + ry * ry + rz * rz), 1e-12f);
+        const float nrm = ray_length(rx, ry, rz);
         u[0] = rx / nrm; u[1] = ry / nrm; u[2] = rz / nrm;
     }
     float enc[32], venc[16];
@@ -793,7 +793,7 @@ __global__ __launch_bounds__(256, 1) void mlp_bwd_dx_fast_kernel(FastBwdArgs a) 
     const long long ri = mc / a.S;
     const float d = a.depth[mc];
     const float rx = a.ray[ri * 3], ry = a.ray[ri * 3 + 1], rz = a.ray[ri * 3 + 2];
-    const float nrm = fmaxf(sqrtf(rx * rx + ry * ry + rz * rz), 1e-12f);
+    const float nrm = ray_length(rx, ry, rz);
     const float ux = rx / nrm, uy = ry / nrm, uz = rz / nrm;
     const float dot = ux * du[0] + uy * du[1] + uz * du[2];
     float gc[3] = {dp[0], dp[1], dp[2]};

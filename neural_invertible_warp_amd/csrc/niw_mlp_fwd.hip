@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256, 1) void mlp_fwd_kernel(MlpFwdArgs a) {
         p[0] = add_rn(a.center[ri * 3 + 0], mul_rn(rx, d));
         p[1] = add_rn(a.center[ri * 3 + 1], mul_rn(ry, d));
         p[2] = add_rn(a.center[ri * 3 + 2], mul_rn(rz, d));
-        const float nrm = fmaxf(sqrtf(rx * rx + ry * ry + rz * rz), 1e-12f);
+        const float nrm = ray_length(rx, ry, rz);
         u[0] = rx / nrm; u[1] = ry / nrm; u[2] = rz / nrm;
     }
     NIW_STAMP(11);                                   // inputs of the sample are in registers; the encodings follow

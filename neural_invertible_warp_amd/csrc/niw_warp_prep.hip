@@ -149,8 +149,9 @@ __global__ __launch_bounds__(256) void warp_prep_bwd_kernel(const float* __restr
     float n2[kRowsPerWave], dot[kRowsPerWave];
 #pragma unroll
     for (int r = 0; r < kRowsPerWave; ++r) {
-        n2[r] = e[r] * e[r] + y0r[r] * y0r[r] + y1r[r] * y1r[r];
-        dot[r] = de[r] * e[r] + dwl0[r] * y0r[r] + dwl1[r] * y1r[r];
+        // (what is fused is stated: no choice of the compiler's)
+        n2[r] = fmaf(y1r[r], y1r[r], fmaf(y0r[r], y0r[r], e[r] * e[r]));
+        dot[r] = fmaf(dwl1[r], y1r[r], fmaf(dwl0[r], y0r[r], de[r] * e[r]));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {

@@ -23,15 +23,11 @@ CSRC = os.path.join(ROOT, "neural_invertible_warp_amd", "csrc")
 # kernels launched with an LDS request that admits ONE workgroup per CU, if any (none at present: the fast-precision kernels, which had the
 # pair, now pass their row offsets through the descriptor and store with soffset 0, which the compiler pads)
 ONE_WORKGROUP_PER_CU_BY_LDS = ()
-# compiled with packed fp32 instructions, like in csrc/Makefile (which says why)
-KEEP_PACKED = ("niw_mlp_", "niw_warp")
 
 
 def compile_to_asm(src, out):
     cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", f"-I{ROOT}/include", f"-I{CSRC}", "-mllvm",
-           "-amdgpu-mfma-vgpr-form", "-S", "--cuda-device-only", src, "-o", out]
-    if not any(os.path.basename(src).startswith(k) for k in KEEP_PACKED):
-        cmd += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+           "-amdgpu-mfma-vgpr-form", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only", src, "-o", out]
     subprocess.run(cmd, check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
     return out
 
