@@ -301,7 +301,7 @@ def _check_tensor(t, name):
         raise _lib.NiwError(f"{name}: expected a strided tensor that holds its own values, got {t.layout}{', a negated view' if t.is_neg() else ''}")
 
 
-_T, _DTYPE, _LAYOUT = torch.Tensor, operator.attrgetter("dtype"), operator.attrgetter("layout")
+_T, _DTYPE, _LAYOUT, _BASE = torch.Tensor, operator.attrgetter("dtype"), operator.attrgetter("layout"), operator.attrgetter("_base")
 
 
 def _gather(tensors, name):
@@ -403,9 +403,10 @@ class _Table:
     """Device image of a list of tensors (niw_table).  The image is stored on the stream that is current when the table is built; a table that
     is kept (`kept`) waits for that once, so that any stream may use it afterwards."""
 
-    def _build(self, name, rows, how, entries, tensors, kept):
+    def _build(self, name, rows, how, entries, tensors, kept, writes):
         lib = _lib.load()
         self._keep = [tensors, [t.untyped_storage() for t in tensors]]
+        self._writes, self._counted = writes, None
         host = np.empty(max(lib.niw_table_bytes(len(rows)), 16), np.uint8)
         image = ctypes.c_void_p(host.ctypes.data)
         self._c = _lib.Table()
@@ -423,6 +424,16 @@ class _Table:
                 self._streams.add(stream.cuda_stream)
                 if kept:
                     stream.synchronize()
+
+    def _wrote(self):
+        """counts a call's writes in the version counters of what was written (`_writes`), as in-place torch operations do: a backward through
+        a saved tensor that the call overwrote is an error then.  Views count in what they are views of -- a bucket's once; tensors of their
+        own cost 50 ns each.  (A graph's replays count nothing, like any replay's.)"""
+        if self._counted is None:
+            owners = {id(t): t for t in (t if base is None else base for t, base in zip(self._writes, map(_BASE, self._writes)))}
+            self._counted = [t for t in owners.values() if not t.is_inference()]
+        if self._counted:
+            torch.autograd.graph.increment_version(self._counted)
 
     def _use(self):
         """the current stream of the list's GPU (its handle alone: a torch.cuda.Stream object costs 2.5 us of a 14 us call), which the image is
@@ -469,12 +480,12 @@ class TensorTable(_Table):
         kept = TABLE_KEPT if _kept else 0
         self._unclippable = None
         try:
-            self._build("niw_grad_table", rows, (TABLE_CLIP | kept,), len(tensors), every, _kept)
+            self._build("niw_grad_table", rows, (TABLE_CLIP | kept,), len(tensors), every, _kept, out if given else tensors)
         except _lib.NiwError as e:
             if given or "overlap" not in str(e):
                 raise
             self._unclippable = str(e)               # tensors that share memory have a norm, but cannot be clipped in place
-            self._build("niw_grad_table", rows, (kept,), len(tensors), every, _kept)
+            self._build("niw_grad_table", rows, (kept,), len(tensors), every, _kept, [])
 
 
 def _table(grads, out=None):
@@ -547,6 +558,7 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None, total=None):
         ws = _norm_workspace(norm.device) if total is None else None
         with timed("clip_grads", table.numel):
             _lib.call("niw_grad_clip", ctypes.byref(table._c), kind, max_norm, _p(total), _p(ws), _p(norm), table._use())
+            table._wrote()
     return norm
 
 
@@ -603,7 +615,8 @@ class AdamTable(_Table):
         self.device = _check_device(tensors, "AdamTable")
         self.n_groups = len(groups)
         self.numel = sum(lengths)
-        self._build("niw_adam_table", rows, (self.n_groups, TABLE_KEPT if _kept else 0), len(lengths), tensors, _kept)
+        self._build("niw_adam_table", rows, (self.n_groups, TABLE_KEPT if _kept else 0), len(lengths), tensors, _kept,
+                    [t for key in names if key != "grads" for t in cols[key]] + masters)
 
 
 def _per_group(value, n, name, kind):
@@ -635,6 +648,7 @@ def adam_step_tensors(tensors, lr, step, weight_decay=0.0, beta1=0.9, beta2=0.99
         with _on(table.device), timed("adam", table.numel):
             _lib.call("niw_adam_step_tensors", ctypes.byref(table._c), hyper, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev), None,
                       table._use())
+            table._wrote()
         return None
     (total, device), kind, max_norm = _total(total, table.device), _norm_kind(norm_type), _max_norm(max_norm)
     with _on(device):
@@ -645,6 +659,7 @@ def adam_step_tensors(tensors, lr, step, weight_decay=0.0, beta1=0.9, beta2=0.99
         with timed("adam", table.numel):
             _lib.call("niw_adam_step_tensors", ctypes.byref(table._c), hyper, float(beta1), float(beta2), float(eps), _p(hyper_dev), _p(decay_dev),
                       ctypes.byref(clip), table._use())
+            table._wrote()
     return norm
 
 
