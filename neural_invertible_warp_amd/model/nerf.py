@@ -391,6 +391,7 @@ class Model:
     reference builds them (the parameters are ordinary nn.Parameters, views of the flat buffers the kernels read).  Checkpoints are
     the reference's model.ckpt dict either way (graph, optim, sched, epoch, iter).  Logging back-ends are outside the path."""
 
+    clip_norm = None      # (what setup_optimizer reads from optim.clip_norm; a subclass with one of its own does not clip)
     grad_norm = None      # torch.optim path under optim.clip_norm: global gradient norm of the last iteration (0-d device tensor)
     trainer = None        # engine.NeRFTrainer when build_networks chose the engine (subclasses that build their own graph keep the torch path)
 
