@@ -5,7 +5,7 @@
 //   niw_adam_step_tensors   Adam by c g, with decoupled weight decay, without ever writing c g
 //
 // All are streams of memory -- 2 flops per element for the norm, 3 for clipping, about 18 for Adam -- and move the algorithm's bytes: the
-// norm 4 GB of fp32 at 7.1 TB/s and 0.67 GB of bf16 at 6.8, a clip 4 GB at 6.2, an update 9.4 GB at 6.3 (a large fill reaches 6.9, a
+// norm 4 GB of fp32 at 7.1 TB/s and 0.67 GB of bf16 at 6.6, a clip 4 GB at 6.2, an update 9.4 GB at 6.3 (a large fill reaches 6.9, a
 // large copy 6.3).  Small lists are bound by two dependent launches of 4 and 6 to 10 us.
 //
 // The list lies in device memory (the image: one slot per tensor that has elements), so a call is one launch over all tensors, however
@@ -445,7 +445,7 @@ struct AdamArgs {
 };
 
 // The update, one part of 1024 elements per workgroup: four elements of every stream per thread, 28 to 30 bytes each, and nothing reused.
-// 335 M bf16 parameters with master copies 1489 us, 101 M fp32 with fp16 gradients in unaligned tensors 408 us.
+// 335 M bf16 parameters with master copies 1483 us, 101 M fp32 with fp16 gradients in unaligned tensors 417 us.
 // DECAY: some group of the call decays (groups that do not then have keep = {1, 2^-100}, which changes no bit).
 template <int KIND, bool NT, bool DECAY>
 __global__ __launch_bounds__(kThreads) void adam_tensors_kernel(List<AdamSlot> list, AdamArgs a, Clip clip) {
