@@ -119,7 +119,7 @@ if __name__ == "__main__":
     ap.add_argument("--seeds", type=int, nargs="+", default=[0, 1])
     ap.add_argument("--variants", nargs="+", default=["base", "randperm", "torch_adam", "per_channel", "rotation_x5", "translation_x5", "views_16"])
     ap.add_argument("--out", default="gpurun_out/plateau.json")
-    ap.add_argument("--hip-graph", action="store_true", help="replay the captured iteration (faster at these small shapes; same numbers bit for bit)")
+    ap.add_argument("--hip-graph", action="store_true", help="replay the captured iteration (refused while engine.REPLAY_OFF stands; same numbers bit for bit)")
     ap.add_argument("--precision", default="fp32", choices=["fp32", "bf16x3", "bf16"])
     ap.add_argument("--log-every", type=int, default=0)
     a = ap.parse_args()
